@@ -609,6 +609,31 @@ int ri_branch_norm_add_norm(float* residual, void* act, int act_dtype, const voi
                             const float* gain, const float* bias, float eps, int kind, const float* layer_scale,
                             const float* next_gain, float next_eps, int tiled, int rows, int dim, void* stream);
 
+// out[m, n] = sum over groups g of scales[n, g] * sum over k in g of x[m, k] (codes[n, k] - zeros[n, g]), m < rows.  codes: uint8
+// [n, k / 2], a byte holds two neighbouring columns, the even one in its low four bits; scales [n, ceil(k / group)] of scale_dtype;
+// zeros uint8 of the same shape, or NULL: 8.  k is a multiple of 8, group 32, 64 or a multiple of 128 (the last may be short).
+int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const void* codes, const void* scales, int scale_dtype,
+                      const void* zeros, int rows, int n, int k, int group, void* stream);
+
+// Attention of the new tokens of `seqs` sequences (cu_seqlens, at most max_new each) whose page tables begin with the same
+// shared_pages pages (read from the first row of page_table); bfloat16, pages of 32, every sequence at most max_len tokens long after
+// the step.  workspace: ri_attention_shared_slots(...) * tokens * heads * (head_dim + 2) floats.  Tokens that are no sequence's
+// (before cu_seqlens[0], from cu_seqlens[seqs] on) get zeros.
+int ri_attention_shared_slots(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads);
+int ri_attention_shared_bf16(void* out, void* workspace, const void* q, int q_stride, const void* k_pages, const void* v_pages,
+                             const int32_t* cu_seqlens, const int32_t* tok_pos, const int32_t* page_table, int table_width,
+                             int num_pages, int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads,
+                             int kv_heads, int head_dim, int page_size, float scale, void* stream);
+
+// Drafted tokens held to the target's distribution (verify.hip): sequence b's rows are cu_seqlens[b] .. cu_seqlens[b + 1] of logits
+// [rows, vocab], row r judges the draft tokens[r + 1]; draft_logits [rows, vocab] or NULL: row j is what tokens[j] was drawn
+// from.  uniform [rows] (NULL with a temperature that is not positive).  accepted [seqs]: drafts that stand; out [rows]: they,
+// the token after them, -1 behind.
+long ri_verify_drafts_workspace_bytes(int seqs, int rows, int vocab);
+int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* logits, const float* draft_logits, const int32_t* tokens,
+                     const int32_t* cu_seqlens, const float* uniform, void* workspace, int seqs, int rows, int vocab,
+                     double temperature, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

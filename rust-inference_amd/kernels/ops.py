@@ -217,6 +217,12 @@ _SIGNATURES = {
                          c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p],
     "ri_ssd_scan_chunked": [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
                             c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, ctypes.c_long, c_void_p],
+    "ri_gemm_int4_bf16": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "ri_attention_shared_slots": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
+    "ri_attention_shared_bf16": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+    "ri_verify_drafts": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                         ctypes.c_double, c_void_p],
     "ri_group_rms_norm": [c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_void_p],
 }
 
@@ -272,6 +278,16 @@ def _dev(t: torch.Tensor, name: str, dtype=None, shape=None) -> int:
 
 def _opt(t, name: str, dtype=None, shape=None):
     return None if t is None else _dev(t, name, dtype, shape)
+
+
+def _on_current_device(*tensors) -> None:
+    """The operands (None among them) lie on one GPU, the current one: a launch goes to that device's stream."""
+    devices = {t.device for t in tensors if isinstance(t, torch.Tensor)}
+    if len(devices) > 1:
+        raise ShapeError(f"the operands lie on {len(devices)} devices: {', '.join(sorted(map(str, devices)))}")
+    for d in devices:
+        if d.type == "cuda" and d.index != torch._C._cuda_getDevice():
+            raise KernelError(f"the operands lie on {d}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
 # ---------------------------------------------------------------- row-wise
@@ -506,6 +522,48 @@ def sample(logits: torch.Tensor, uniform, temperature: float, top_k: int = 0, to
           _opt(uniform, "uniform", torch.float32, (rows,)), rows, vocab, float(temperature), int(top_k), float(top_p),
           float(penalty), _stream())
     return out
+
+
+def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.Tensor, uniform, temperature: float,
+                  draft_logits: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Drafted tokens held to the target's distribution: a step that was fed ``tokens`` (int32 ``[rows]``, sequence ``b``'s at
+    ``cu_seqlens[b]..cu_seqlens[b + 1]``: its last known token, then its drafts, none of them or any number) and whose logits
+    are all wanted.  Row ``r`` of float32 ``logits [rows, vocab]`` is what follows token ``r`` and judges the draft
+    ``tokens[r + 1]``: with ``p = softmax(logits[r] / temperature)`` and ``q`` the distribution the draft was drawn from it
+    stands if ``uniform[r] * q(draft) < p(draft)``.  ``draft_logits`` (float32 ``[rows, vocab]``): row ``j`` is what ``tokens[j]`` was
+    drawn from, at the same temperature (rows of tokens that are no drafts are not read); None: the drafts were not drawn
+    (looked up), ``q`` is 1 at the draft.  Behind the drafts that stand comes one more token, drawn with the number of the
+    sequence's last row: from ``max(p - q, 0)`` where a draft fell, else from the last row's ``p``; the first token whose running
+    weight, by rising id, passes the number times the weight of all.  With a temperature that is not positive a draft stands while
+    it is the row's best token (the first of equal ones), and the row's best token follows.
+
+    Returns int32 ``accepted [seqs]``, the drafts that stand, and int32 ``out [rows]``, at the sequence's rows the drafts that stand, the
+    token after them, then -1 (also in rows that are no sequence's).  NaN and -inf mask an entry (a target cut to its best
+    entries is given so), an infinite logit counts as the largest finite number; a draft outside the vocabulary falls.  A row that
+    masks everything lets no draft stand and gives token 0.  At most 65,535 rows and sequences."""
+    if logits.dim() != 2:
+        raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise ShapeError(f"cu_seqlens must be [seqs + 1], got {list(cu_seqlens.shape)}")
+    seqs, temperature = cu_seqlens.shape[0] - 1, float(temperature)
+    if rows < 1 or vocab < 1:
+        raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
+    if temperature > 0 and uniform is None:
+        raise ShapeError("a temperature above 0 wants uniform numbers, one a row")
+    _on_current_device(logits, tokens, cu_seqlens, uniform, draft_logits)
+    args = (_dev(logits, "logits", torch.float32), _opt(draft_logits, "draft_logits", torch.float32, (rows, vocab)),
+            _dev(tokens, "tokens", torch.int32, (rows,)), _dev(cu_seqlens, "cu_seqlens", torch.int32),
+            _opt(uniform, "uniform", torch.float32, (rows,)))
+    lib = load()
+    lib.ri_verify_drafts_workspace_bytes.restype = ctypes.c_long
+    lib.ri_verify_drafts_workspace_bytes.argtypes = [c_int, c_int, c_int]
+    ws = torch.empty((lib.ri_verify_drafts_workspace_bytes(seqs, rows, vocab),), dtype=torch.uint8, device=logits.device)
+    accepted = torch.empty((seqs,), dtype=torch.int32, device=logits.device)
+    out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    _call("ri_verify_drafts", _dev(accepted, "accepted"), _dev(out, "out"), *args, _dev(ws, "workspace"), seqs, rows, vocab, temperature,
+          _stream())
+    return accepted, out
 
 
 def mark_seen(seen: torch.Tensor, rows: torch.Tensor, tokens: torch.Tensor) -> None:
@@ -1424,6 +1482,40 @@ def attention_decode_fused_bf16(qkv, q_gain, k_gain, eps, inv_freq, k_pages, v_p
     return out
 
 
+def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table, seqs: int, max_new: int, shared: int, max_len: int,
+                          heads: int, kv_heads: int, head_dim: int, scale: float, q_off: int = 0) -> torch.Tensor:
+    """Matrix-core attention for a batch whose sequences begin with the same ``shared`` tokens in the same pages: what
+    ``attention_prefill_bf16`` and ``attention_decode_bf16`` compute without a window, with the shared pages read once for all new
+    tokens instead of once a sequence.  ``shared`` is a multiple of the page (32 tokens; 0: nothing is shared) and the first
+    ``shared / 32`` entries of every row of ``page_table`` are the same pages (the first row's are read).  Any number of new tokens
+    a sequence, at most ``max_new`` (one, or a drafted step's few); their keys and values are in the cache.  ``max_len`` bounds every
+    sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  ``q_off`` as in
+    ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
+    tokens, stride = qkv.shape
+    num_pages, hkv, page_size, dh = k_pages.shape
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ShapeError(f"attention: {heads} heads over {kv_heads} kv heads")
+    if (hkv, dh) != (kv_heads, head_dim) or tuple(v_pages.shape) != (num_pages, hkv, dh, page_size):
+        raise ShapeError(f"pages are {list(k_pages.shape)} / {list(v_pages.shape)}, the mixer has {kv_heads} kv heads of {head_dim}")
+    if q_off < 0 or q_off + heads * head_dim > stride or q_off % 8:
+        raise ShapeError(f"attention: queries at column {q_off} of rows of {stride} for {heads} heads of {head_dim}")
+    if shared < 0 or shared % page_size:
+        raise ShapeError(f"attention: {shared} shared tokens are no whole pages of {page_size}")
+    if page_table.dim() != 2 or page_table.shape[0] < seqs:
+        raise ShapeError(f"page_table is {list(page_table.shape)} for {seqs} sequences")
+    _on_current_device(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table)
+    args = (_dev(qkv, "qkv", torch.bfloat16) + 2 * int(q_off), stride, _dev(k_pages, "k_pages", torch.bfloat16),
+            _dev(v_pages, "v_pages", torch.bfloat16), _dev(cu_seqlens, "cu_seqlens", torch.int32, (seqs + 1,)),
+            _dev(tok_pos, "tok_pos", torch.int32, (tokens,)), _dev(page_table, "page_table", torch.int32))
+    first = shared // page_size
+    slots = _get("ri_attention_shared_slots")(tokens, seqs, int(max_new), first, int(max_len), heads, kv_heads)
+    ws = torch.empty((max(slots, 1) * tokens * heads * (head_dim + 2),), dtype=torch.float32, device=qkv.device)
+    out = torch.empty((tokens, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
+    _call("ri_attention_shared_bf16", _dev(out, "out"), _dev(ws, "workspace"), *args, page_table.shape[1], num_pages, tokens, seqs,
+          int(max_new), first, int(max_len), heads, kv_heads, head_dim, page_size, float(scale), _stream())
+    return out
+
+
 # ---------------------------------------------------------------- products
 def gemm_f32(x: torch.Tensor, w: torch.Tensor, tile: int = -1) -> torch.Tensor:
     """``x @ w.T`` with no input rounded and float32 sums; ``x`` float32 ``[M, K]``, ``w`` float32 or bfloat16 ``[N, K]``.
@@ -1462,6 +1554,29 @@ def pack_for_mfma(w: torch.Tensor, swiglu: bool = False) -> torch.Tensor:
         w = padded
     tiles = w.view(n16 // 16, 16, k32 // 32, 4, 8).permute(0, 2, 3, 1, 4)      # [row tile, k tile, k group, row, 8]
     return tiles.reshape(n16 // 16, k32 // 32, 64, 8).contiguous()
+
+
+def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group: int, zeros: torch.Tensor | None = None,
+                   out_dtype=torch.bfloat16) -> torch.Tensor:
+    """``x @ w.T`` for bfloat16 rows ``x [M, K]`` and a matrix in 4 bits: ``w[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k //
+    group])``.  ``codes`` (uint8 ``[N, K / 2]``) hold two neighbouring columns a byte, the even one in the low four bits; ``scales``
+    (bfloat16 or float32) and ``zeros`` (uint8; None: 8 everywhere) are ``[N, ceil(K / group)]``.  ``group`` is 32, 64 or a multiple of
+    128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights; more rows
+    go 64 at a time.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at the end."""
+    if x.dim() != 2 or codes.dim() != 2:
+        raise ShapeError(f"x and codes are matrices, got {list(x.shape)} and {list(codes.shape)}")
+    (m, k), n = x.shape, codes.shape[0]
+    if group not in (32, 64) and (group < 1 or group % 128):
+        raise ShapeError(f"groups of {group} columns: 32, 64 and multiples of 128 are taken")
+    if m < 1 or n < 1 or k < 8 or k % 8:
+        raise ShapeError(f"a product of {m} rows, {n} columns and k {k}: at least one each, k a multiple of 8")
+    groups = -(-k // group)
+    _on_current_device(x, codes, scales, zeros)
+    out = torch.empty((m, n), dtype=out_dtype, device=x.device)
+    _call("ri_gemm_int4_bf16", _dev(out, "out"), code(out_dtype), _dev(x, "x", torch.bfloat16), _dev(codes, "codes", torch.uint8, (n, k // 2)),
+          _dev(scales, "scales", None, (n, groups)), code(scales.dtype), _opt(zeros, "zeros", torch.uint8, (n, groups)), m, n, k, int(group),
+          _stream())
+    return out
 
 
 TILED_X, TILED_OUT = 1, 2
