@@ -628,8 +628,8 @@ int ri_attention_shared_bf16(void* out, void* workspace, const void* q, int q_st
 // Drafted tokens held to the target's distribution (verify.hip): sequence b's rows are cu_seqlens[b] .. cu_seqlens[b + 1] of logits
 // [rows, vocab], row r judges the draft tokens[r + 1]; draft_logits [rows, vocab] or NULL: row j is what tokens[j] was drawn
 // from.  uniform [rows] (NULL with a temperature that is not positive).  accepted [seqs]: drafts that stand; out [rows]: they,
-// the token after them, -1 behind.
-long ri_verify_drafts_workspace_bytes(int seqs, int rows, int vocab);
+// the token after them, -1 behind.  workspace: that many numbers of 8 bytes (0: refused).
+int ri_verify_drafts_workspace_words(int seqs, int rows, int vocab, int with_draft);
 int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* logits, const float* draft_logits, const int32_t* tokens,
                      const int32_t* cu_seqlens, const float* uniform, void* workspace, int seqs, int rows, int vocab,
                      double temperature, void* stream);

@@ -122,6 +122,11 @@ static inline typename std::common_type<A, B>::type max(A a, B b) {
 }
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
+// v_med3_f32: the middle of three; where one is NaN the least of the others.
+static inline float emu_med3(float a, float b, float c) {
+    return a != a ? fminf(b, c) : b != b ? fminf(a, c) : c != c ? fminf(a, b) : fmaxf(fminf(a, b), fminf(fmaxf(a, b), c));
+}
+#define __builtin_amdgcn_fmed3f(a, b, c) emu_med3((a), (b), (c))
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
 
 // ---- atomics: one host thread runs everything

@@ -12,14 +12,13 @@
 //
 // Everything that is compared is held in 64 bits: a token is the answer to "on which side of a border does u lie", a
 // vocabulary has 10^5 borders, and float32 weights put one draw in 10^3 to 10^5 on the wrong side.  The vector unit takes
-// float64 at the rate of float32, so it is the polynomial of exp2_nonpositive, 17 instructions an entry, that stands beside
-// the 4 bytes of it.
+// float64 well, so that an exponential of thirteen instructions (Exps, below) stands beside an entry's 4 bytes.
 //
-// Three launches.  `stats` cuts every row that is asked about into chunks of 4,096 entries, a workgroup each, and leaves a
-// chunk's largest logit and its sum of exponentials: the one pass over the logits.  `weigh` (a workgroup a chunk of the
-// vocabulary and sequence) joins the rows' chunks in order until a draft falls, which every workgroup of a sequence does
-// for itself (a few kilobytes), and sums its chunk of the row that the last token is drawn from.  `pick` (a workgroup a
-// sequence) finds the chunk and in it the token.  Greedy steps need two: the chunks' best entries, then the walk.
+// Four launches.  `stats` cuts every row that is asked about into chunks of 4,096 entries, a wavefront each, and leaves a
+// chunk's largest logit and its sum of exponentials: the one pass over the logits.  `end` (a workgroup a sequence) joins the
+// rows' chunks, a row a wavefront, until a draft falls.  `weigh` sums what the entries of every chunk weigh in the draw
+// of the last token, `pick` (a workgroup a sequence) finds the chunk and in it the token.  Greedy steps need two: the
+// chunks' best entries, then the walk.
 // Every sum has one order, so the same inputs give the same tokens.
 #include <float.h>
 
@@ -29,12 +28,12 @@
 #define VER_CHUNK 4096
 #define VER_THREADS 256
 #define VER_WAVES (VER_THREADS / RI_WAVE)
-#define VER_EACH (VER_CHUNK / VER_THREADS)
 #define VER_PICK_THREADS 1024
 #define VER_PICK_EACH (VER_CHUNK / VER_PICK_THREADS)
 
-struct ChunkStats { double top, sum; };          // of a chunk of a row: its largest logit, the sum of exp((x - top) / T)
-struct RowStats { double top, inv; };            // of a row: its largest logit, 1 / the sum (0 where every entry is masked)
+// With s = log2(e) / T, the exponential of a logit x over that of the largest one m is 2^((x - m) s).
+struct ChunkStats { double top, sum; };          // of a chunk of a row: m, the sum over its entries
+struct RowStats { double top, inv; };            // of a row: m, 1 / the sum (0 where every entry is masked)
 // Where a sequence's walk ended: the row that the last token is drawn from, the draft that fell there (-1: none did, or it
 // has a distribution of its own), and the statistics of both distributions.
 struct Ending {
@@ -42,27 +41,70 @@ struct Ending {
     int row, less, fell, unused;
 };
 
-// 2^t for t <= 0 (t NaN: 0), relative error under 3e-13: t = n + f with |f| <= 1/2, the Taylor sum of e^(f ln 2) up to the
-// tenth power (the next term is 0.3466^11 / 11! = 2.2e-13), times 2^n.
+#define VER_MAGIC 6755399441055744.0             // 1.5 * 2^52: a number added to it is rounded to a whole one, in the lowest bits
+
+// 2^f for |f| <= 1/2 times 2^n, n the low 32 bits of `whole`: the polynomial of degree 8 that equals 2^f at the nine Chebyshev
+// points of [-1/2, 1/2] (relative error under 1.1e-12); n is added to the exponent, which has to have room for it.
+__device__ __forceinline__ double exp2_parts(double f, double whole) {
+    double s = 1.3255224878668817e-06;
+    s = fma(s, f, 1.5310079402249296e-05);
+    s = fma(s, f, 0.00015403455852453838);
+    s = fma(s, f, 0.0013333450568000645);
+    s = fma(s, f, 0.0096181291594025584);
+    s = fma(s, f, 0.055504109412059327);
+    s = fma(s, f, 0.24022650695812989);
+    s = fma(s, f, 0.69314718054593349);
+    s = fma(s, f, 1.0);
+    typedef uint32_t __attribute__((ext_vector_type(2))) halves_t;
+    halves_t bits = __builtin_bit_cast(halves_t, s);
+    bits.y += __builtin_bit_cast(halves_t, whole).x << 20;
+    return __builtin_bit_cast(double, bits);
+}
+// 2^t for t <= 0: t = n + f by adding and taking off 1.5 * 2^52.  t is held to -1000 (NaN with it), where 2^t is 1e-301, nothing
+// beside a sum of at least 1.
 __device__ __forceinline__ double exp2_nonpositive(double t) {
-    t = fmax(t, -1100.0);
-    const double n = rint(t), z = (t - n) * 0.69314718055994530942;
-    double s = 1.0 / 3628800.0;
-    s = fma(s, z, 1.0 / 362880.0);
-    s = fma(s, z, 1.0 / 40320.0);
-    s = fma(s, z, 1.0 / 5040.0);
-    s = fma(s, z, 1.0 / 720.0);
-    s = fma(s, z, 1.0 / 120.0);
-    s = fma(s, z, 1.0 / 24.0);
-    s = fma(s, z, 1.0 / 6.0);
-    s = fma(s, z, 0.5);
-    s = fma(s, z, 1.0);
-    s = fma(s, z, 1.0);
-    return ldexp(s, (int)n);
+    t = fmin(fmax(t, -1000.0), 0.0);
+    const double y = t + VER_MAGIC;
+    return exp2_parts(t - (y - VER_MAGIC), y);
 }
 
-// A logit as the sampled forms take it: NaN is a masked entry, an infinite one the largest finite number.
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : fminf(x, FLT_MAX); }
+// The exponentials of a row's (or a chunk's) entries over that of its largest one.  Ordinary temperatures: with M the whole
+// number next to m s, 2^(x s - M) takes thirteen float64 instructions, since x s + (1.5 * 2^52 - M) has the whole part in
+// place at once, and x is held in float32 to what the exponent has room for: lo, where the result is 2^-1000 up to the
+// rounding of lo.  That wants |M| below 2^27; `plain` does without.  NaN and what lies at lo or below is a masked entry, an
+// infinite logit the largest finite number.
+struct Scale { double s, inv; };                 // log2(e) / T and its inverse
+struct Exps {
+    double s, c, back;           // log2(e) / T; 1.5 * 2^52 - M; 2^(M - m s)
+    float top, lo;
+    bool plain;
+};
+__device__ __forceinline__ Exps exps_below(double m, Scale by) {
+    Exps r;
+    const double whole = rint(m * by.s);
+    r.s = by.s;
+    r.top = (float)m;
+    r.plain = !(fabs(whole) < 134217728.0);
+    r.c = VER_MAGIC - whole;
+    r.lo = (float)((whole - 1000.0) * by.inv);
+    r.back = r.plain ? 1.0 : exp2_parts(fma(-m, by.s, whole), 0.0);
+    return r;
+}
+// What `back` times it is the exponential of x.
+template <bool PLAIN>
+__device__ __forceinline__ double term(const Exps& r, float x) {
+    if (PLAIN) return exp2_nonpositive(((double)x - (double)r.top) * r.s);
+    const double d = __builtin_amdgcn_fmed3f(x, r.lo, r.top);           // (with a NaN the least of the others)
+    const double y = fma(d, r.s, r.c);
+    return exp2_parts(fma(d, r.s, r.c - y), y);
+}
+// The same with 0 for a masked entry, where it matters whether an entry weighs anything at all.
+template <bool PLAIN>
+__device__ __forceinline__ double term_or_zero(const Exps& r, float x) {
+    const double e = term<PLAIN>(r, x);
+    const bool some = PLAIN ? ((double)x - (double)r.top) * r.s > -1000.0 || x > r.top : x > r.lo;
+    return some ? e : 0.0;
+}
 
 __device__ __forceinline__ double wave_sum_d(double v) {
 #pragma unroll
@@ -77,12 +119,26 @@ __device__ __forceinline__ double wave_max_d(double v) {
 
 // A thread's entries of a chunk of n entries; those that are not there are masked.  WIDE: the row starts on a 16-byte
 // boundary and its length is a multiple of 4.
-template <bool WIDE>
-__device__ __forceinline__ void load_chunk(float (&v)[VER_EACH], const float* __restrict__ x, int n) {
+template <bool WIDE, int EACH>
+__device__ __forceinline__ void load_chunk(float (&v)[EACH], const float* __restrict__ x, int n) {
+    constexpr int THREADS = VER_CHUNK / EACH;
+    if (n == VER_CHUNK) {                                     // (all chunks but a row's last: no looks at the end)
+        if (WIDE) {
+#pragma unroll
+            for (int u = 0; u < EACH / 4; ++u) {
+                const float4 w = *reinterpret_cast<const float4*>(x + 4 * (u * THREADS + threadIdx.x));
+                v[4 * u] = w.x, v[4 * u + 1] = w.y, v[4 * u + 2] = w.z, v[4 * u + 3] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < EACH; ++u) v[u] = x[u * THREADS + threadIdx.x];
+        }
+        return;
+    }
     if (WIDE) {
 #pragma unroll
-        for (int u = 0; u < VER_EACH / 4; ++u) {
-            const int i = 4 * (u * VER_THREADS + threadIdx.x);
+        for (int u = 0; u < EACH / 4; ++u) {
+            const int i = 4 * (u * THREADS + threadIdx.x);
             const float4 w = *reinterpret_cast<const float4*>(x + min(i, n - 4));
             v[4 * u] = i < n ? w.x : -INFINITY;
             v[4 * u + 1] = i < n ? w.y : -INFINITY;
@@ -91,17 +147,18 @@ __device__ __forceinline__ void load_chunk(float (&v)[VER_EACH], const float* __
         }
     } else {
 #pragma unroll
-        for (int u = 0; u < VER_EACH; ++u) {
-            const int i = u * VER_THREADS + threadIdx.x;
+        for (int u = 0; u < EACH; ++u) {
+            const int i = u * THREADS + threadIdx.x;
             const float w = x[min(i, n - 1)];
             v[u] = i < n ? w : -INFINITY;
         }
     }
 }
 // The place in its chunk of a thread's entry e.
-template <bool WIDE>
+template <bool WIDE, int EACH>
 __device__ __forceinline__ int place_of(int e) {
-    return WIDE ? 4 * ((e / 4) * VER_THREADS + threadIdx.x) + e % 4 : e * VER_THREADS + threadIdx.x;
+    constexpr int THREADS = VER_CHUNK / EACH;
+    return WIDE ? 4 * ((e / 4) * THREADS + threadIdx.x) + e % 4 : e * THREADS + threadIdx.x;
 }
 
 // The rows of a sequence, held to the rows there are.
@@ -124,106 +181,117 @@ __device__ __forceinline__ void place_of_row(const int32_t* __restrict__ cu, int
     drafted = within && !__any(first);
 }
 
+// A chunk a wavefront, 64 entries a lane: what is done once a wavefront (place, reductions) is a fifth of its instructions so, a
+// third with 32.  The vector unit bounds this pass nearly as the memory does.
 template <bool WIDE>
-__global__ __launch_bounds__(VER_THREADS) void verify_stats(ChunkStats* __restrict__ stats, const float* __restrict__ logits,
-                                                            const float* __restrict__ draft, const int32_t* __restrict__ cu,
-                                                            int seqs, int rows, int vocab, int chunks, double scale) {
-    const int chunk = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
+__global__ __launch_bounds__(RI_WAVE) void verify_stats(ChunkStats* __restrict__ stats, const float* __restrict__ logits,
+                                                        const float* __restrict__ draft, const int32_t* __restrict__ cu, int seqs,
+                                                        int rows, int vocab, int chunks, Scale scale) {
+    constexpr int EACH = VER_CHUNK / RI_WAVE;
+    const int chunk = blockIdx.x, row = blockIdx.y;
     const bool of_draft = blockIdx.z == 1;
-    __shared__ double shared[2 * VER_WAVES];
     const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
-    float v[VER_EACH];
+    float v[EACH];
     load_chunk<WIDE>(v, (of_draft ? draft : logits) + (size_t)row * vocab + at, n);
     bool within, drafted;
     place_of_row(cu, seqs, rows, row, within, drafted);
-    if (of_draft ? !drafted : !within) return;                // the whole workgroup: nobody asks about this row
-    float top = -INFINITY;
+    if (of_draft ? !drafted : !within) return;                // nobody asks about this row
+    float top = -INFINITY;                                    // (the larger of a number and NaN is the number)
 #pragma unroll
-    for (int e = 0; e < VER_EACH; ++e) {
-        v[e] = clean(v[e]);
-        top = fmaxf(top, v[e]);
-    }
+    for (int e = 0; e < EACH; ++e) top = fmaxf(top, v[e]);
     top = wave_max(top);
-    if (lane == 0) shared[wave] = top;
-    __syncthreads();
-    double m = shared[0];
+    const double m = fminf(top, FLT_MAX);
+    const Exps r = exps_below(m, scale);
+    double sum = 0.0, more = 0.0;
+    if (r.plain) {
 #pragma unroll
-    for (int w = 1; w < VER_WAVES; ++w) m = fmax(m, shared[w]);
-    double sum = 0.0;
+        for (int e = 0; e < EACH; ++e) sum += term<true>(r, v[e]);
+    } else {
 #pragma unroll
-    for (int e = 0; e < VER_EACH; ++e) sum += exp2_nonpositive(((double)v[e] - m) * scale);
-    sum = wave_sum_d(sum);
-    if (lane == 0) shared[VER_WAVES + wave] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double s = shared[VER_WAVES];
-#pragma unroll
-        for (int w = 1; w < VER_WAVES; ++w) s += shared[VER_WAVES + w];
-        stats[((size_t)blockIdx.z * rows + row) * chunks + chunk] = {m, s};
+        for (int e = 0; e < EACH; e += 2) {
+            sum += term<false>(r, v[e]);
+            more += term<false>(r, v[e + 1]);
+        }
     }
+    sum = wave_sum_d(sum + more) * r.back;
+    if (threadIdx.x == 0) stats[((size_t)blockIdx.z * rows + row) * chunks + chunk] = {m, top > -INFINITY ? sum : 0.0};
 }
 
 // A row's chunks joined, by a wavefront, in an order that the number of chunks alone decides.
-__device__ __forceinline__ RowStats join_row(const ChunkStats* __restrict__ c, int chunks, double scale) {
+__device__ __forceinline__ RowStats join_row(const ChunkStats* __restrict__ c, int chunks, Scale scale) {
     const int lane = threadIdx.x & (RI_WAVE - 1);
     double m = -INFINITY;
     for (int i = lane; i < chunks; i += RI_WAVE) m = fmax(m, c[i].top);
     m = wave_max_d(m);
     double s = 0.0;
-    for (int i = lane; i < chunks; i += RI_WAVE) s += c[i].sum * exp2_nonpositive((c[i].top - m) * scale);
+    for (int i = lane; i < chunks; i += RI_WAVE) s += c[i].sum * exp2_nonpositive((c[i].top - m) * scale.s);
     s = wave_sum_d(s);
     return {m, s > 0.0 ? 1.0 / s : 0.0};
 }
 
-__device__ __forceinline__ double probability(const RowStats s, float x, double scale) {
-    return exp2_nonpositive(((double)clean(x) - s.top) * scale) * s.inv;
+__device__ __forceinline__ double probability(const RowStats s, float x, Scale scale) {
+    const Exps r = exps_below(s.top, scale);
+    return (r.plain ? term_or_zero<true>(r, x) : term_or_zero<false>(r, x)) * r.back * s.inv;
 }
 
 // What an entry weighs in the last draw: first in the distribution that is left, second in p itself (taken where nothing is
 // left, as when p and q are equal up to their rounding).
 struct Weights { double left, whole; };
-__device__ __forceinline__ Weights weigh_entry(const Ending& e, float x, float qx, bool has_q, int id, double scale) {
-    const double p = probability(e.p, x, scale);
-    double left = p;
-    if (e.fell) left = has_q ? fmax(p - probability(e.q, qx, scale), 0.0) : id == e.less ? 0.0 : p;
-    return {left, p};
+struct Weigher {
+    Exps p, q;
+    double p_inv, q_inv;
+    int less;                    // the entry that a fallen draft without a distribution takes out, -1: none
+    bool has_q, plain;           // plain: one of the two wants it, both are taken so
+};
+__device__ __forceinline__ Weigher weigher(const Ending& e, bool with_draft, Scale scale) {
+    Weigher w;
+    w.has_q = with_draft && e.fell;
+    w.p = exps_below(e.p.top, scale);
+    w.q = exps_below(w.has_q ? e.q.top : e.p.top, scale);
+    w.plain = w.p.plain || w.q.plain;
+    w.p_inv = w.plain ? e.p.inv : w.p.back * e.p.inv;
+    w.q_inv = w.plain ? e.q.inv : w.q.back * e.q.inv;
+    w.less = e.fell && !with_draft ? e.less : -1;
+    return w;
+}
+template <bool PLAIN, bool HAS_Q>
+__device__ __forceinline__ Weights weigh_entry(const Weigher& w, float x, float qx, int id) {
+    const double p = term_or_zero<PLAIN>(w.p, x) * w.p_inv;
+    if (HAS_Q) return {fmax(fma(-w.q_inv, term_or_zero<PLAIN>(w.q, qx), p), 0.0), p};
+    return {id == w.less ? 0.0 : p, p};
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(VER_THREADS) void verify_weigh(Weights* __restrict__ masses, Ending* __restrict__ endings,
-                                                            const ChunkStats* __restrict__ stats, const float* __restrict__ logits,
-                                                            const float* __restrict__ draft, const int32_t* __restrict__ tokens,
-                                                            const int32_t* __restrict__ cu, const float* __restrict__ uniform,
-                                                            int rows, int vocab, int chunks, double scale) {
-    const int chunk = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
+__global__ __launch_bounds__(VER_THREADS) void verify_end(Ending* __restrict__ endings, const ChunkStats* __restrict__ stats,
+                                                          const float* __restrict__ logits, const float* __restrict__ draft,
+                                                          const int32_t* __restrict__ tokens, const int32_t* __restrict__ cu,
+                                                          const float* __restrict__ uniform, int rows, int vocab, int chunks, Scale scale) {
+    const int b = blockIdx.x, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
     __shared__ Ending tried[VER_WAVES];
-    __shared__ Weights sums[VER_WAVES];
     int r0, r1;
     rows_of(cu, b, rows, r0, r1);
     if (r0 == r1) return;
     // four rows at a time, a wavefront each, until one ends the walk; the last row always does
-    Ending end;
     for (int base = r0;; base += VER_WAVES) {
         const int row = base + wave;
         Ending mine = {{0.0, 0.0}, {0.0, 0.0}, -1, -1, 0, 0};
         if (row < r1) {
+            const bool last = row == r1 - 1;
+            const int d = last ? -1 : tokens[row + 1];
+            const bool known = d >= 0 && d < vocab;           // a draft that is no token of the vocabulary falls
+            const float x = logits[(size_t)row * vocab + (known ? d : 0)];
+            float qx = 0.f;
+            if (draft && !last) {
+                qx = draft[(size_t)(row + 1) * vocab + (known ? d : 0)];
+                mine.q = join_row(stats + ((size_t)rows + row + 1) * chunks, chunks, scale);
+            }
             mine.p = join_row(stats + (size_t)row * chunks, chunks, scale);
-            if (row == r1 - 1) {
+            const double p = known ? probability(mine.p, x, scale) : 0.0;
+            const double q = !known ? 0.0 : draft ? probability(mine.q, qx, scale) : 1.0;
+            const bool stands = (double)uniform[row] * q < p;
+            if (last || !stands) {
                 mine.row = row;
-            } else {
-                const int d = tokens[row + 1];
-                const bool known = d >= 0 && d < vocab;       // a draft that is no token of the vocabulary falls
-                double q = 1.0;
-                if (draft) {
-                    mine.q = join_row(stats + ((size_t)rows + row + 1) * chunks, chunks, scale);
-                    q = known ? probability(mine.q, draft[(size_t)(row + 1) * vocab + d], scale) : 0.0;
-                }
-                const double p = known ? probability(mine.p, logits[(size_t)row * vocab + d], scale) : 0.0;
-                if (!((double)uniform[row] * q < p)) {
-                    mine.row = row;
-                    mine.less = d;
-                    mine.fell = 1;
-                }
+                mine.less = d;
+                mine.fell = !last;
             }
         }
         if (lane == 0) tried[wave] = mine;
@@ -232,23 +300,46 @@ __global__ __launch_bounds__(VER_THREADS) void verify_weigh(Weights* __restrict_
         for (int w = VER_WAVES - 1; w >= 0; --w)
             if (tried[w].row >= 0) first = w;
         if (first >= 0) {
-            end = tried[first];
-            break;
+            if (threadIdx.x == 0) endings[b] = tried[first];
+            return;
         }
         __syncthreads();
     }
-    if (chunk == 0 && threadIdx.x == 0) endings[b] = end;
-    const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
-    const bool has_q = draft != nullptr;
-    float x[VER_EACH], qx[VER_EACH];
-    load_chunk<WIDE>(x, logits + (size_t)end.row * vocab + at, n);
-    if (has_q && end.fell) load_chunk<WIDE>(qx, draft + (size_t)(end.row + 1) * vocab + at, n);
+}
+
+template <bool PLAIN, bool HAS_Q, bool WIDE, int EACH>
+__device__ __forceinline__ Weights sum_weights(const Weigher& by, const float (&x)[EACH], const float (&qx)[EACH], int at) {
     Weights sum = {0.0, 0.0};
 #pragma unroll
-    for (int e = 0; e < VER_EACH; ++e) {
-        const Weights w = weigh_entry(end, x[e], qx[e], has_q, at + place_of<WIDE>(e), scale);
+    for (int e = 0; e < EACH; ++e) {
+        const Weights w = weigh_entry<PLAIN, HAS_Q>(by, x[e], qx[e], at + place_of<WIDE, EACH>(e));
         sum.left += w.left;
         sum.whole += w.whole;
+    }
+    return sum;
+}
+
+template <bool WIDE>
+__global__ __launch_bounds__(VER_THREADS) void verify_weigh(Weights* __restrict__ masses, const Ending* __restrict__ endings,
+                                                            const float* __restrict__ logits, const float* __restrict__ draft,
+                                                            const int32_t* __restrict__ cu, int rows, int vocab, int chunks, Scale scale) {
+    constexpr int EACH = VER_CHUNK / VER_THREADS;
+    const int chunk = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
+    __shared__ Weights sums[VER_WAVES];
+    int r0, r1;
+    rows_of(cu, b, rows, r0, r1);
+    if (r0 == r1) return;
+    const Ending end = endings[b];
+    const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
+    const Weigher by = weigher(end, draft != nullptr, scale);
+    float x[EACH], qx[EACH];
+    load_chunk<WIDE>(x, logits + (size_t)end.row * vocab + at, n);
+    Weights sum;
+    if (by.has_q) {
+        load_chunk<WIDE>(qx, draft + (size_t)(end.row + 1) * vocab + at, n);
+        sum = by.plain ? sum_weights<true, true, WIDE>(by, x, qx, at) : sum_weights<false, true, WIDE>(by, x, qx, at);
+    } else {
+        sum = by.plain ? sum_weights<true, false, WIDE>(by, x, x, at) : sum_weights<false, false, WIDE>(by, x, x, at);
     }
     sum.left = wave_sum_d(sum.left);
     sum.whole = wave_sum_d(sum.whole);
@@ -276,16 +367,60 @@ __device__ __forceinline__ void put_out(int32_t* __restrict__ accepted, int32_t*
     }
 }
 
+// A wavefront's values with all lanes' before them added, in the order that the steps fix.
+__device__ __forceinline__ double wave_upto(double v) {
+    const int lane = threadIdx.x & (RI_WAVE - 1);
+#pragma unroll
+    for (int d = 1; d < RI_WAVE; d *= 2) {
+        const double o = __shfl(v, max(lane - d, 0), RI_WAVE);
+        v += lane >= d ? o : 0.0;
+    }
+    return v;
+}
+
+// Where the draw falls among a sequence's chunks: the first whose running weight passes the target, else the last that weighs
+// anything; what the chunks before it weigh.  By a wavefront, a lane a chunk.
+struct Drawn { double target, before; int chunk, whole; };
+__device__ __forceinline__ Drawn draw_chunk(const Weights* __restrict__ mine, int chunks, double u) {
+    const int lane = threadIdx.x & (RI_WAVE - 1);
+    double left = 0.0, whole = 0.0;                           // of all chunks
+    for (int c0 = 0; c0 < chunks; c0 += RI_WAVE) {
+        const Weights w = c0 + lane < chunks ? mine[c0 + lane] : Weights{0.0, 0.0};
+        left += __shfl(wave_upto(w.left), RI_WAVE - 1, RI_WAVE);
+        whole += __shfl(wave_upto(w.whole), RI_WAVE - 1, RI_WAVE);
+    }
+    Drawn d;
+    d.whole = !(left > 0.0);
+    d.target = u * (d.whole ? whole : left);
+    d.before = 0.0;
+    d.chunk = 0;
+    double carried = 0.0;
+    for (int c0 = 0; c0 < chunks; c0 += RI_WAVE) {
+        const Weights w = c0 + lane < chunks ? mine[c0 + lane] : Weights{0.0, 0.0};
+        const double own = d.whole ? w.whole : w.left, upto = carried + wave_upto(own);
+        const unsigned long long some = __ballot(own > 0.0), past = __ballot(own > 0.0 && upto > d.target);
+        const unsigned long long take = past ? past & (0ull - past) : some;       // the first past the target, else the last of some
+        if (take) {
+            const int who = 63 - __clzll((long long)take);
+            d.chunk = c0 + who;
+            d.before = who > 0 ? __shfl(upto, max(who - 1, 0), RI_WAVE) : carried;
+        }
+        if (past) break;
+        carried = __shfl(upto, RI_WAVE - 1, RI_WAVE);
+    }
+    return d;
+}
+
 __global__ __launch_bounds__(VER_PICK_THREADS) void verify_pick(int32_t* __restrict__ accepted, int32_t* __restrict__ out,
                                                                 const Weights* __restrict__ masses, const Ending* __restrict__ endings,
                                                                 const float* __restrict__ logits, const float* __restrict__ draft,
                                                                 const int32_t* __restrict__ tokens, const int32_t* __restrict__ cu,
                                                                 const float* __restrict__ uniform, int seqs, int rows, int vocab,
-                                                                int chunks, double scale) {
+                                                                int chunks, Scale scale) {
+    constexpr int WAVES = VER_PICK_THREADS / RI_WAVE;
     const int b = blockIdx.x, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
-    __shared__ double upto_wave[VER_PICK_THREADS / RI_WAVE];
-    __shared__ double before_chunk;
-    __shared__ int chosen, whole, found, last_some;
+    __shared__ double of_wave[WAVES];
+    __shared__ int first_past[WAVES], last_some[WAVES];
     int r0, r1;
     rows_of(cu, b, rows, r0, r1);
     if (r0 == r1) {
@@ -293,77 +428,46 @@ __global__ __launch_bounds__(VER_PICK_THREADS) void verify_pick(int32_t* __restr
         return;
     }
     const Ending end = endings[b];
-    const Weights* mine = masses + (size_t)b * chunks;
-    const double u = uniform[r1 - 1];
-    if (threadIdx.x == 0) {
-        double left = 0.0, all = 0.0;
-        for (int c = 0; c < chunks; ++c) {
-            left += mine[c].left;
-            all += mine[c].whole;
-        }
-        const int take_all = !(left > 0.0);
-        const double target = u * (take_all ? all : left);
-        double upto = 0.0, before = 0.0, before_some = 0.0;
-        int at = -1, some = 0;
-        for (int c = 0; c < chunks; ++c) {
-            const double w = take_all ? mine[c].whole : mine[c].left;
-            if (w > 0.0) {
-                some = c;
-                before_some = upto;
-            }
-            upto += w;
-            if (upto > target) {
-                at = c;
-                before = before_some;
-                break;
-            }
-        }
-        chosen = at < 0 ? some : at;                          // (nothing passes: u is not below 1)
-        before_chunk = at < 0 ? before_some : before;
-        whole = take_all;
-        found = VER_CHUNK;
-        last_some = -1;
-        upto_wave[0] = target;
-    }
-    __syncthreads();
-    const double target = upto_wave[0];
-    const int at = chosen * VER_CHUNK, n = min(VER_CHUNK, vocab - at), first = threadIdx.x * VER_PICK_EACH;
-    const bool has_q = draft != nullptr;
+    const Drawn d = draw_chunk(masses + (size_t)b * chunks, chunks, uniform[r1 - 1]);       // (every wavefront for itself)
+    const int at = d.chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at), first = threadIdx.x * VER_PICK_EACH;
+    const Weigher by = weigher(end, draft != nullptr, scale);
     double w[VER_PICK_EACH], sum = 0.0;
 #pragma unroll
     for (int e = 0; e < VER_PICK_EACH; ++e) {
         const int i = first + e, id = at + min(i, n - 1);
         const float x = logits[(size_t)end.row * vocab + id];
-        const float qx = has_q && end.fell ? draft[(size_t)(end.row + 1) * vocab + id] : 0.f;
-        const Weights ws = weigh_entry(end, x, qx, has_q, id, scale);
-        w[e] = i < n ? (whole ? ws.whole : ws.left) : 0.0;
+        const float qx = by.has_q ? draft[(size_t)(end.row + 1) * vocab + id] : 0.f;
+        const Weights ws = by.has_q ? by.plain ? weigh_entry<true, true>(by, x, qx, id) : weigh_entry<false, true>(by, x, qx, id)
+                                    : by.plain ? weigh_entry<true, false>(by, x, qx, id) : weigh_entry<false, false>(by, x, qx, id);
+        w[e] = i < n ? (d.whole ? ws.whole : ws.left) : 0.0;
         sum += w[e];
     }
-    double upto = sum;                                        // of the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < RI_WAVE; d *= 2) {
-        const double o = __shfl(upto, max(lane - d, 0), RI_WAVE);
-        upto += lane >= d ? o : 0.0;
-    }
-    __syncthreads();                                          // everybody has read the target
-    if (lane == RI_WAVE - 1) upto_wave[wave] = upto;
+    const double upto = wave_upto(sum);
+    if (lane == RI_WAVE - 1) of_wave[wave] = upto;
     __syncthreads();
-    double before = before_chunk;
-    for (int v = 0; v < wave; ++v) before += upto_wave[v];
-    double run = before + (upto - sum);
+    double run = d.before;
+    for (int v = 0; v < wave; ++v) run += of_wave[v];
+    run += upto - sum;
+    int past = -1, some = -1;                                 // of this thread's entries
+#pragma unroll
+    for (int e = VER_PICK_EACH - 1; e >= 0; --e)
+        if (w[e] > 0.0 && some < 0) some = first + e;
 #pragma unroll
     for (int e = 0; e < VER_PICK_EACH; ++e) {
         run += w[e];
-        if (w[e] > 0.0) atomicMax(&last_some, first + e);     // (whole numbers: the order of the lanes changes nothing)
-        if (w[e] > 0.0 && run > target) {
-            atomicMax(&found, VER_CHUNK * 2 - (first + e));   // the first such place, counted from behind
-            break;
-        }
+        if (w[e] > 0.0 && run > d.target && past < 0) past = first + e;
     }
+    const unsigned long long pasts = __ballot(past >= 0), somes = __ballot(some >= 0);
+    if (pasts ? lane == __builtin_ctzll(pasts) : lane == 0) first_past[wave] = past;
+    if (somes ? lane == 63 - __clzll((long long)somes) : lane == 0) last_some[wave] = some;
     __syncthreads();
     // (the chunk's sum and its entries' running sum are added up in another order: a target within their rounding of the
     // chunk's end falls to its last entry that weighs anything)
-    const int place = found > VER_CHUNK ? VER_CHUNK * 2 - found : max(last_some, 0);
+    int place = 0;
+    for (int v = 0; v < WAVES; ++v)
+        if (last_some[v] >= 0) place = last_some[v];
+    for (int v = WAVES - 1; v >= 0; --v)
+        if (first_past[v] >= 0) place = first_past[v];
     put_out(accepted, out, tokens, cu, seqs, rows, b, r0, r1, end.row, at + place);
 }
 
@@ -386,12 +490,13 @@ __global__ __launch_bounds__(VER_THREADS) void verify_best(Best* __restrict__ be
     const int chunk = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
     __shared__ Best shared[VER_WAVES];
     const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
-    float v[VER_EACH];
+    constexpr int EACH = VER_CHUNK / VER_THREADS;
+    float v[EACH];
     load_chunk<WIDE>(v, logits + (size_t)row * vocab + at, n);
     Best best = {-INFINITY, at};                              // (a chunk of masked entries names its first)
 #pragma unroll
-    for (int e = 0; e < VER_EACH; ++e)
-        if (v[e] > best.value) best = {v[e], at + place_of<WIDE>(e)};      // (by rising place; NaN is above nothing)
+    for (int e = 0; e < EACH; ++e)
+        if (v[e] > best.value) best = {v[e], at + place_of<WIDE, EACH>(e)};      // (by rising place; NaN is above nothing)
     best = wave_best(best);
     if (lane == 0) shared[wave] = best;
     __syncthreads();
@@ -435,10 +540,13 @@ __global__ __launch_bounds__(VER_THREADS) void verify_walk(int32_t* __restrict__
 
 static inline int verify_chunks(int vocab) { return (vocab + VER_CHUNK - 1) / VER_CHUNK; }
 
-extern "C" long ri_verify_drafts_workspace_bytes(int seqs, int rows, int vocab) {
-    if (seqs < 1 || rows < 1 || vocab < 1) return 0;
+// Numbers of 8 bytes; 0: such a call is refused (or its workspace would pass 16 GB).
+extern "C" int ri_verify_drafts_workspace_words(int seqs, int rows, int vocab, int with_draft) {
+    if (seqs < 1 || rows < 1 || vocab < 1 || vocab > 0x7fffffff - VER_CHUNK) return 0;
     const long chunks = verify_chunks(vocab);
-    return 2L * rows * chunks * (long)sizeof(ChunkStats) + seqs * chunks * (long)sizeof(Weights) + seqs * (long)sizeof(Ending);
+    const long bytes = (with_draft ? 2L : 1L) * rows * chunks * (long)sizeof(ChunkStats) + seqs * chunks * (long)sizeof(Weights) +
+                       seqs * (long)sizeof(Ending);
+    return bytes / 8 <= 0x7fffffffL ? (int)(bytes / 8) : 0;
 }
 
 extern "C" int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* logits, const float* draft_logits, const int32_t* tokens,
@@ -446,7 +554,8 @@ extern "C" int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* lo
                                 double temperature, void* stream) {
     RI_REQUIRE(seqs >= 1 && rows >= 1 && vocab >= 1, "verify_drafts: %d sequences, %d rows, a vocabulary of %d", seqs, rows, vocab);
     RI_REQUIRE(rows <= 65535 && seqs <= 65535, "verify_drafts: %d rows of %d sequences, at most 65535 go in one call", rows, seqs);
-    RI_REQUIRE(vocab <= 0x7fffffff - VER_CHUNK, "verify_drafts: a vocabulary of %d is too large", vocab);
+    RI_REQUIRE(ri_verify_drafts_workspace_words(seqs, rows, vocab, draft_logits != nullptr) > 0,
+               "verify_drafts: %d rows of a vocabulary of %d are too much for one call", rows, vocab);
     RI_REQUIRE(accepted && out && logits && tokens && cu_seqlens && workspace, "verify_drafts: an operand is missing");
     RI_REQUIRE(temperature == temperature, "verify_drafts: the temperature is no number");
     const hipStream_t s = (hipStream_t)stream;
@@ -463,19 +572,16 @@ extern "C" int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* lo
     }
     RI_REQUIRE(uniform, "verify_drafts: a temperature above 0 wants the random numbers");
     ChunkStats* stats = (ChunkStats*)workspace;
-    Weights* masses = (Weights*)(stats + 2L * rows * chunks);
+    Weights* masses = (Weights*)(stats + (draft_logits ? 2L : 1L) * rows * chunks);
     Ending* endings = (Ending*)(masses + (long)seqs * chunks);
-    const double scale = fmin(1.4426950408889634074 / temperature, 1e300);       // (finite: 0 times it is 0)
+    const double by = fmin(1.4426950408889634074 / temperature, 1e200);       // (a difference of logits times it stays finite)
+    const Scale scale = {by, 1.0 / by};
     const dim3 grid(chunks, rows, draft_logits ? 2 : 1), grid2(chunks, seqs);
-    if (wide) {
-        verify_stats<true><<<grid, VER_THREADS, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
-        verify_weigh<true><<<grid2, VER_THREADS, 0, s>>>(masses, endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, rows,
-                                                         vocab, chunks, scale);
-    } else {
-        verify_stats<false><<<grid, VER_THREADS, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
-        verify_weigh<false><<<grid2, VER_THREADS, 0, s>>>(masses, endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, rows,
-                                                          vocab, chunks, scale);
-    }
+    if (wide) verify_stats<true><<<grid, RI_WAVE, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
+    else verify_stats<false><<<grid, RI_WAVE, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
+    verify_end<<<seqs, VER_THREADS, 0, s>>>(endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, rows, vocab, chunks, scale);
+    if (wide) verify_weigh<true><<<grid2, VER_THREADS, 0, s>>>(masses, endings, logits, draft_logits, cu_seqlens, rows, vocab, chunks, scale);
+    else verify_weigh<false><<<grid2, VER_THREADS, 0, s>>>(masses, endings, logits, draft_logits, cu_seqlens, rows, vocab, chunks, scale);
     verify_pick<<<seqs, VER_PICK_THREADS, 0, s>>>(accepted, out, masses, endings, logits, draft_logits, tokens, cu_seqlens, uniform, seqs,
                                                   rows, vocab, chunks, scale);
     RI_LAUNCH_CHECK("verify_drafts");

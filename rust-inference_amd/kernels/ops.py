@@ -221,6 +221,7 @@ _SIGNATURES = {
     "ri_attention_shared_slots": [c_int, c_int, c_int, c_int, c_int, c_int, c_int],
     "ri_attention_shared_bf16": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                  c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p],
+    "ri_verify_drafts_workspace_words": [c_int, c_int, c_int, c_int],
     "ri_verify_drafts": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                          ctypes.c_double, c_void_p],
     "ri_group_rms_norm": [c_void_p, c_int, c_void_p, c_void_p, c_float, c_int, c_int, c_int, c_void_p],
@@ -280,14 +281,14 @@ def _opt(t, name: str, dtype=None, shape=None):
     return None if t is None else _dev(t, name, dtype, shape)
 
 
-def _on_current_device(*tensors) -> None:
+def _on_current_device(first: torch.Tensor, *others) -> None:
     """The operands (None among them) lie on one GPU, the current one: a launch goes to that device's stream."""
-    devices = {t.device for t in tensors if isinstance(t, torch.Tensor)}
-    if len(devices) > 1:
-        raise ShapeError(f"the operands lie on {len(devices)} devices: {', '.join(sorted(map(str, devices)))}")
-    for d in devices:
-        if d.type == "cuda" and d.index != torch._C._cuda_getDevice():
-            raise KernelError(f"the operands lie on {d}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    at = first.get_device()                                   # (-1: not on a GPU, which the check of every operand refuses)
+    for t in others:
+        if t is not None and t.get_device() != at:
+            raise ShapeError(f"the operands lie on {first.device} and {t.device}")
+    if at >= 0 and at != torch._C._cuda_getDevice():
+        raise KernelError(f"the operands lie on {first.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
 # ---------------------------------------------------------------- row-wise
@@ -555,10 +556,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     args = (_dev(logits, "logits", torch.float32), _opt(draft_logits, "draft_logits", torch.float32, (rows, vocab)),
             _dev(tokens, "tokens", torch.int32, (rows,)), _dev(cu_seqlens, "cu_seqlens", torch.int32),
             _opt(uniform, "uniform", torch.float32, (rows,)))
-    lib = load()
-    lib.ri_verify_drafts_workspace_bytes.restype = ctypes.c_long
-    lib.ri_verify_drafts_workspace_bytes.argtypes = [c_int, c_int, c_int]
-    ws = torch.empty((lib.ri_verify_drafts_workspace_bytes(seqs, rows, vocab),), dtype=torch.uint8, device=logits.device)
+    ws = torch.empty((_get("ri_verify_drafts_workspace_words")(seqs, rows, vocab, int(draft_logits is not None)),), dtype=torch.float64,
+                     device=logits.device)
     accepted = torch.empty((seqs,), dtype=torch.int32, device=logits.device)
     out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
     _call("ri_verify_drafts", _dev(accepted, "accepted"), _dev(out, "out"), *args, _dev(ws, "workspace"), seqs, rows, vocab, temperature,

@@ -394,6 +394,21 @@ def test_drafts_are_verified(ops, counts, vocab, temperature, with_draft):
              plain_verify(logits, draft, tokens, counts, u, temperature))
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 1e-12, 1e-8, 1e-6, 1e-3, 50.0, 1e6, 1e30])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_temperatures_at_the_ends_of_their_range(ops, temperature, with_draft):
+    """Cold: everything falls to the largest logit; hot: all entries weigh alike."""
+    counts, vocab = [3, 2, 5], 4500
+    logits, draft, tokens, u = drafted(counts, vocab, 1.0, with_draft, 12)
+    best = logits.argmax(1)
+    tokens[1], tokens[6], tokens[7] = best[0], best[5], best[6]
+    if with_draft:
+        draft[[1, 6, 7], tokens[[1, 6, 7]]] = 9.0
+    with np.errstate(over="ignore"):
+        want = plain_verify(logits, draft, tokens, counts, u, temperature, margin=1e-9)
+    same(verify(ops, logits, draft, tokens, counts, u, temperature), want)
+
+
 @pytest.mark.parametrize("vocab", [411, 5000])
 def test_drafts_of_the_target_itself_all_stand(ops, vocab):
     counts = [6, 1, 9]
