@@ -51,87 +51,281 @@ __device__ __forceinline__ void drop_behind(PageFrags<DH>& f, int last, int lane
     }
 }
 
-// A tile of 16 columns over a run of pages, the pages in turn among the wavefronts.
 template <int DH>
-__global__ void __launch_bounds__(SH_WAVES * 64) attn_shared_kernel(const SharedArgs a) {
-    constexpr int LD = DH + 4;
-    __shared__ __attribute__((aligned(16))) float o_lds[SH_WAVES][16 * LD];
-    __shared__ float m_lds[SH_WAVES][16], l_lds[SH_WAVES][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, jg = lane >> 4;
-    const int kvh = blockIdx.y, group = a.heads / a.kv_heads;
-    const int shared_items = a.splits * a.tiles;
-    int slot, col0, cols, first_token, page0, page1, last_key;
-    const int32_t* table = a.page_table;
-    if ((int)blockIdx.x < shared_items) {
-        slot = blockIdx.x / a.tiles;
-        first_token = 0;
-        cols = a.tokens * group;
-        col0 = (blockIdx.x % a.tiles) * 16;
-        page0 = slot * a.pages_per_split;
-        page1 = min(page0 + a.pages_per_split, a.shared_pages);
-        last_key = a.shared_pages * PAGE - 1;
-    } else {
-        int item = blockIdx.x - shared_items;
-        const int chunk = item % a.own_chunks;
-        item /= a.own_chunks;
-        const int seq = item / a.own_tiles;
-        slot = a.splits + chunk;
-        first_token = min(max(a.cu_seqlens[seq], 0), a.tokens);
-        const int behind = min(max(a.cu_seqlens[seq + 1], first_token), a.tokens);
-        cols = (behind - first_token) * group;
-        col0 = (item % a.own_tiles) * 16;
-        if (col0 >= cols) return;
-        last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
-        page0 = a.shared_pages + chunk * SH_OWN_PAGES;
-        page1 = min(page0 + SH_OWN_PAGES, last_key / PAGE + 1);
-        if (page0 >= page1) return;
-        table += (size_t)seq * a.table_width;
-    }
+struct SharedLds {
+    static constexpr int LD = DH + 4;                        // a column's stride, floats
+    union {
+        struct { bf16_t k[PAIR_SLOTS][2][PAGE * DH], v[PAIR_SLOTS][2][PAGE * DH]; } pages;
+        struct { float o[SH_WAVES][16 * LD], m[SH_WAVES][16], l[SH_WAVES][16]; } meet;
+    };
+};
+
+// Column `col` of the tokens first_token ..: its token and query head.
+struct Place { int token, head; };
+__device__ __forceinline__ Place place_of(const SharedArgs& a, int first_token, int kvh, int col) {
+    const int group = a.heads / a.kv_heads, t = col / group;
+    return {first_token + t, kvh * group + col - t * group};
+}
+__device__ __forceinline__ size_t result_at(const SharedArgs& a, int slot, Place p) {
+    return ((size_t)slot * a.tokens + p.token) * a.heads + p.head;
+}
+
+// Few columns: a tile of 16 over the pages page0 .. page1, which the wavefronts take in turn, each the next page on its way while it
+// weighs one; they meet in LDS.
+template <int DH>
+__device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& lds, const int32_t* table, int kvh, int slot,
+                                            int first_token, int col0, int cols, int page0, int page1, int last_key) {
+    constexpr int LD = SharedLds<DH>::LD;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
     Columns<DH, 1> c;
     init_columns<DH, 1>(c);
-    const int col = col0 + i, token = first_token + col / group, head = kvh * group + col % group;
-    if (col < cols) {
-        c.qpos[0] = min(a.tok_pos[token], last_key);
-        const bf16_t* q = a.q + (size_t)token * a.q_stride + head * DH + jg * 8;
+    const int col = col0 + i;
+    const Place place = place_of(a, first_token, kvh, min(col, cols - 1));
+    c.qpos[0] = min(a.tok_pos[place.token], last_key);
+    const bf16_t* q = a.q + (size_t)place.token * a.q_stride + place.head * DH + jg * 8;
 #pragma unroll
-        for (int ks = 0; ks < DH / 32; ++ks) c.q[0][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
-    }
-    for (int page = page0 + wave; page < page1; page += SH_WAVES) {
-        const long phys = min(max(table[page], 0), a.num_pages - 1);
-        PageFrags<DH> f;
-        load_page<DH>(f, a.k_pages, a.v_pages, phys, a.kv_heads, kvh, lane);
+    for (int ks = 0; ks < DH / 32; ++ks) c.q[0][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
+    auto load = [&](PageFrags<DH>& f, int page) {            // (behind the last page: a line of it)
+        const int p = min(page, page1 - 1);
+        load_page<DH>(f, a.k_pages, a.v_pages, min(max(table[p], 0), a.num_pages - 1), a.kv_heads, kvh, lane, page < page1);
+    };
+    auto take = [&](PageFrags<DH>& f, int page) {
         const int last = last_key - page * PAGE;
         if (last < PAGE - 1) drop_behind<DH>(f, last, lane);
-        const bool open = !__any(col < cols && c.qpos[0] < page * PAGE + PAGE - 1);
-        process_page<DH, 1>(c, f, page, lane, a.scale_log2, open);
+        process_page<DH, 1>(c, f, page, lane, a.scale_log2, !__any(c.qpos[0] < page * PAGE + PAGE - 1));
+    };
+    PageFrags<DH> even, odd;
+    int page = page0 + wave;
+    if (page < page1) {
+        load(even, page);
+        for (;; page += 2 * SH_WAVES) {
+            load(odd, page + SH_WAVES);
+            take(even, page);
+            if (page + SH_WAVES >= page1) break;
+            load(even, page + 2 * SH_WAVES);
+            take(odd, page + SH_WAVES);
+            if (page + 2 * SH_WAVES >= page1) break;
+        }
     }
     finish_columns<DH, 1>(c);
+    auto& meet = lds.meet;
     if (jg == 0) {
-        m_lds[wave][i] = c.m[0];
-        l_lds[wave][i] = c.l[0];
+        meet.m[wave][i] = c.m[0];
+        meet.l[wave][i] = c.l[0];
     }
     __syncthreads();
-    float m = m_lds[0][i], l = 0.f;
+    float m = meet.m[0][i], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < SH_WAVES; ++w) m = fmaxf(m, m_lds[w][i]);
+    for (int w = 1; w < SH_WAVES; ++w) m = fmaxf(m, meet.m[w][i]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < SH_WAVES; ++w) l += __builtin_amdgcn_exp2f(m_lds[w][i] - ref) * l_lds[w][i];
+    for (int w = 0; w < SH_WAVES; ++w) l += __builtin_amdgcn_exp2f(meet.m[w][i] - ref) * meet.l[w][i];
     const float mine = __builtin_amdgcn_exp2f(c.m[0] - ref);
 #pragma unroll
     for (int dt = 0; dt < DH / 16; ++dt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o_lds[wave][i * LD + dt * 16 + jg * 4 + e] = c.o[0][dt][e] * mine;
-    if (wave == 0 && jg == 0 && col < cols) a.stats[((size_t)slot * a.tokens + token) * a.heads + head] = make_float2(m, l);
+        *reinterpret_cast<float4*>(&meet.o[wave][i * LD + dt * 16 + jg * 4]) =
+            make_float4(c.o[0][dt][0] * mine, c.o[0][dt][1] * mine, c.o[0][dt][2] * mine, c.o[0][dt][3] * mine);
+    if (wave == 0 && jg == 0 && col < cols) a.stats[result_at(a, slot, place)] = make_float2(m, l);
     __syncthreads();
-    for (int at = threadIdx.x; at < 16 * DH; at += SH_WAVES * 64) {
-        const int r = at / DH, d = at % DH, cc = col0 + r;
-        if (cc >= cols) break;
-        float o = o_lds[0][r * LD + d];
+    for (int at = threadIdx.x; at < 16 * DH / 4; at += SH_WAVES * 64) {
+        const int r = at / (DH / 4), d = at % (DH / 4) * 4;
+        if (col0 + r >= cols) break;
+        float4 o = *reinterpret_cast<const float4*>(&meet.o[0][r * LD + d]);
 #pragma unroll
-        for (int w = 1; w < SH_WAVES; ++w) o += o_lds[w][r * LD + d];
-        a.sums[(((size_t)slot * a.tokens + first_token + cc / group) * a.heads + kvh * group + cc % group) * DH + d] = o;
+        for (int w = 1; w < SH_WAVES; ++w) {
+            const float4 more = *reinterpret_cast<const float4*>(&meet.o[w][r * LD + d]);
+            o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
+        }
+        *reinterpret_cast<float4*>(a.sums + result_at(a, slot, place_of(a, first_token, kvh, col0 + r)) * DH + d) = o;
     }
+}
+
+// Many columns: a wavefront takes 16 NT of them and walks all pages page0 .. page1, two at a time (a pair that ends behind page1 takes
+// its last page twice, the second time masked); the pages are copied into LDS once for the four wavefronts, keys of pair u + 2 and values of
+// pair u + 1 while pair u is weighed, one place a turn where the wavefronts meet.
+template <int DH, int NT>
+__device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>& lds, int kvh, int slot, int col0, int cols, int page0, int page1) {
+    typedef CopiedPage<DH> Copied;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
+    const int last_key = page1 * PAGE - 1, u_last = (page1 - page0 - 1) / 2;
+    auto& k_lds = lds.pages.k;
+    auto& v_lds = lds.pages.v;
+    Columns<DH, NT> c;
+    init_columns<DH, NT>(c);
+    int min_qpos = last_key;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int col = min(col0 + (wave * NT + j) * 16 + i, cols - 1);         // (columns behind the last repeat it and are not stored)
+        const Place p = place_of(a, 0, kvh, col);
+        c.qpos[j] = min(a.tok_pos[p.token], last_key);
+        min_qpos = min(min_qpos, c.qpos[j]);
+        const bf16_t* q = a.q + (size_t)p.token * a.q_stride + p.head * DH + jg * 8;
+#pragma unroll
+        for (int ks = 0; ks < DH / 32; ++ks) c.q[j][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
+    }
+    const bool all_seen = !__any(min_qpos < last_key);
+    auto page_of = [&](int u) { return page0 + 2 * u; };
+    auto open = [&](int u) { return all_seen && page_of(u) + 1 < page1; };
+    auto look = [&](int u, int h) -> int {
+        const int phys = a.page_table[min(page_of(min(u, u_last)) + h, page1 - 1)];
+        return min(max(phys, 0), a.num_pages - 1);
+    };
+    uint32_t off[Copied::MINE];
+    Copied::offsets(off, wave, lane);
+    auto fetch_keys = [&](int u, const int (&at)[2]) {       // (wavefronts 0 and 1)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            Copied::copy(ma_lds(k_lds[(unsigned)u % PAIR_SLOTS][h]), off, a.k_pages + ((long)at[h] * a.kv_heads + kvh) * (PAGE * DH), wave);
+    };
+    auto fetch_values = [&](int u, const int (&at)[2]) {     // (wavefronts 2 and 3)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            Copied::copy(ma_lds(v_lds[(unsigned)u % PAIR_SLOTS][h]), off, a.v_pages + ((long)at[h] * a.kv_heads + kvh) * (PAGE * DH), wave - 2);
+    };
+    auto fetch = [&](int u, const int (&k)[2], const int (&v)[2]) {       // keys of pair u, values of pair u - 1
+        if (wave < 2) fetch_keys(u, k);
+        else fetch_values(u - 1, v);
+    };
+    auto scores = [&](float (&s)[NT][2][8], int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Frag kf[2][DH / 32];
+            Copied::keys(kf, k_lds[(unsigned)u % PAIR_SLOTS][h], lane);
+            float one[NT][8];
+            scores_of<DH, NT>(c, kf, one, 0, lane);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[j][h][e] = one[j][e];
+        }
+    };
+    auto mask = [&](float (&s)[NT][2][8], int u) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if ((page_of(u) + e / 8) * PAGE + jg * 8 + e % 8 > c.qpos[j]) s[j][e / 8][e % 8] = -INFINITY;
+    };
+    auto maxima = [&](const float (&s)[NT][2][8], float (&m_new)[NT]) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float mx = s[j][0][0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[j][e / 8][e % 8]);
+            m_new[j] = fmaxf(c.m[j], column_max<(NT >= 2 || DH < 128)>(mx) * a.scale_log2);
+        }
+    };
+    float s_cur[NT][2][8], ref[NT], m_new[NT];
+    int now[2], next[2];                                     // where the pages of pairs u + 1 and u + 2 lie
+    {
+        const int first[2] = {look(0, 0), look(0, 1)};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            now[h] = look(1, h);
+            next[h] = look(2, h);
+        }
+        if (wave < 2) fetch_keys(0, first);
+        fetch(1, now, first);
+    }
+    ma_wait_copies<2 * Copied::MINE>();
+    ma_meet();
+    scores(s_cur, 0);
+    if (!open(0)) mask(s_cur, 0);
+    maxima(s_cur, m_new);
+    move_reference<DH, NT>(c, m_new, ref);
+    auto weights = [&](Frag (&w)[NT], int h) {
+        float one[NT][8];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) one[j][e] = s_cur[j][h][e];
+        weights_of<DH, NT>(c, one, ref, w, a.scale_log2);
+    };
+    auto values = [&](const Frag (&w)[NT], int u, int h) {
+        Frag vf[DH / 16];
+        Copied::values(vf, v_lds[(unsigned)u % PAIR_SLOTS][h], lane);
+        weighted_values<DH, NT>(c, vf, w);
+    };
+    auto turn = [&](int u, auto masked) {                    // u: the pair whose weights are due
+        ma_wait_copies<0>();                                  // the keys of pair u + 1 and the values of pair u are there,
+        ma_wait_lds();                                        // the keys of pair u and the values of pair u - 1 read
+        ma_meet();
+        fetch(u + 2, next, now);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            now[h] = next[h];
+            next[h] = look(u + 3, h);
+        }
+        Frag w[2][NT];
+        float s_next[NT][2][8];
+        scores(s_next, u + 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) weights(w[h], h);
+        if (decltype(masked)::value) mask(s_next, u + 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) values(w[h], u, h);
+        maxima(s_next, m_new);
+        move_reference<DH, NT>(c, m_new, ref);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s_cur[j][e / 8][e % 8] = s_next[j][e / 8][e % 8];
+    };
+    int u = 0;
+    for (; u < u_last && open(u + 1); ++u) turn(u, std::false_type());
+    for (; u < u_last; ++u) turn(u, std::true_type());
+    ma_wait_copies<0>();                                      // (also what was copied for nobody: it must not arrive in another workgroup's LDS)
+    ma_meet();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                            // the last pair's weights and value products
+        Frag w[NT];
+        weights(w, h);
+        values(w, u_last, h);
+    }
+    finish_columns<DH, NT>(c);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int col = col0 + (wave * NT + j) * 16 + i;
+        if (col >= cols) continue;
+        const size_t at = result_at(a, slot, place_of(a, 0, kvh, col));
+        if (jg == 0) a.stats[at] = make_float2(c.m[j], c.l[j]);
+#pragma unroll
+        for (int dt = 0; dt < DH / 16; ++dt)
+            *reinterpret_cast<float4*>(a.sums + at * DH + dt * 16 + jg * 4) = make_float4(c.o[j][dt][0], c.o[j][dt][1], c.o[j][dt][2], c.o[j][dt][3]);
+    }
+}
+
+// NT: tiles of 16 columns a wavefront takes of the shared pages; 0: the wavefronts of a workgroup share one tile.
+// Workgroups by rising number: the shared pages' runs, a tile after the other, so that the tiles that read the same pages lie
+// a multiple of eight apart and meet in one XCD's L2; then the sequences' own chunks.
+template <int DH, int NT>
+__global__ void __launch_bounds__(SH_WAVES * 64, 2) attn_shared_kernel(const SharedArgs a) {
+    __shared__ __attribute__((aligned(16))) SharedLds<DH> lds;
+    const int of_tile = a.splits * a.kv_heads, shared_items = of_tile * a.tiles;
+    int item = blockIdx.x;
+    if (item < shared_items) {
+        const int tile = item / of_tile;
+        item -= tile * of_tile;
+        const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads;
+        const int page0 = slot * a.pages_per_split, page1 = min(page0 + a.pages_per_split, a.shared_pages);
+        const int cols = a.tokens * (a.heads / a.kv_heads);
+        if (NT == 0) few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, cols, page0, page1, a.shared_pages * PAGE - 1);
+        else many_columns<DH, NT == 0 ? 1 : NT>(a, lds, kvh, slot, tile * 64 * NT, cols, page0, page1);
+        return;
+    }
+    item -= shared_items;
+    const int kvh = item % a.kv_heads;
+    item /= a.kv_heads;
+    const int seq = item / (a.own_tiles * a.own_chunks);
+    item -= seq * a.own_tiles * a.own_chunks;
+    const int chunk = item / a.own_tiles, tile = item - chunk * a.own_tiles;
+    const int first = min(max(a.cu_seqlens[seq], 0), a.tokens), behind = min(max(a.cu_seqlens[seq + 1], first), a.tokens);
+    const int cols = (behind - first) * (a.heads / a.kv_heads);
+    if (tile * 16 >= cols) return;
+    const int last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
+    const int page0 = a.shared_pages + chunk * SH_OWN_PAGES, page1 = min(page0 + SH_OWN_PAGES, last_key / PAGE + 1);
+    if (page0 >= page1) return;
+    few_columns<DH>(a, lds, a.page_table + (size_t)seq * a.table_width, kvh, a.splits + chunk, first, tile * 16, cols, page0, page1, last_key);
 }
 
 // A token's runs and chunks joined, a workgroup a (head, token); tokens that are no sequence's get zeros.
@@ -161,18 +355,24 @@ __global__ void __launch_bounds__(DH) attn_shared_join_kernel(bf16_t* __restrict
     *to = f32_to_bf16(l > 0.f ? o / l : 0.f);
 }
 
-struct SharedPlan { int splits, pages_per_split, tiles, own_tiles, own_chunks; };
+struct SharedPlan { int nt, splits, pages_per_split, tiles, own_tiles, own_chunks; };
 
-// Runs of the shared pages: four workgroups a compute unit, eight pages a run at least (two a wavefront).
-static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
+// More than 32 columns a key head take the form of many columns (a tile of 64 or, from 65 columns on, 128 a workgroup).  Runs of
+// the shared pages: two workgroups a compute unit, eight pages a run at least.
+static SharedPlan shared_plan(int tokens, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     SharedPlan p;
     const int group = heads / kv_heads;
-    p.tiles = (int)(((long)tokens * group + 15) / 16);
+    const long cols = (long)tokens * group;
+    p.nt = cols <= 32 ? 0 : cols <= 64 ? 1 : 2;
+    const int of_wg = p.nt == 0 ? 16 : 64 * p.nt;
+    p.tiles = (int)((cols + of_wg - 1) / of_wg);
     p.own_tiles = (int)(((long)max_new * group + 15) / 16);
     const int own = max_len - shared_pages * PAGE;
     p.own_chunks = own > 0 ? (own + SH_OWN_PAGES * PAGE - 1) / (SH_OWN_PAGES * PAGE) : 0;
-    const long wanted = 4L * ri_compute_units() / ((long)p.tiles * kv_heads) + 1;
-    p.pages_per_split = shared_pages ? (int)((shared_pages + wanted - 1) / wanted) : 1;
+    long runs = 2L * ri_compute_units() / ((long)p.tiles * kv_heads);
+    if (runs < 1) runs = 1;
+    p.pages_per_split = (int)((shared_pages + runs - 1) / runs);
+    p.pages_per_split += p.pages_per_split & 1;
     if (p.pages_per_split < 8) p.pages_per_split = 8;
     p.splits = (shared_pages + p.pages_per_split - 1) / p.pages_per_split;
     return p;
@@ -180,7 +380,7 @@ static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_page
 
 extern "C" int ri_attention_shared_slots(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     if (tokens < 1 || seqs < 1 || max_new < 1 || shared_pages < 0 || max_len < 1 || kv_heads < 1 || heads < kv_heads) return 0;
-    const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
+    const SharedPlan p = shared_plan(tokens, max_new, shared_pages, max_len, heads, kv_heads);
     return p.splits + p.own_chunks;
 }
 
@@ -200,20 +400,24 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE((long)table_width * PAGE < 0x7fffffff, "attention_shared: page table width %d", table_width);
     RI_REQUIRE(scale > 0.f, "attention_shared: scale %g is not positive", (double)scale);
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
-    const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
-    const long items = (long)p.splits * p.tiles + (long)p.own_chunks * p.own_tiles * seqs;
-    RI_REQUIRE(items <= 0x7fffffff, "attention_shared: %ld workgroups exceed one launch", items);
+    const SharedPlan p = shared_plan(tokens, max_new, shared_pages, max_len, heads, kv_heads);
+    const long items = ((long)p.splits * p.tiles + (long)p.own_chunks * p.own_tiles * seqs) * kv_heads;
+    RI_REQUIRE(items <= 0x7fffffff / (SH_WAVES * 64), "attention_shared: %ld workgroups exceed one launch", items);
     const size_t rows = (size_t)(p.splits + p.own_chunks) * tokens * heads;
     const SharedArgs a = {(float*)workspace, (float2*)((float*)workspace + rows * head_dim), (const bf16_t*)q, (const bf16_t*)k_pages,
                           (const bf16_t*)v_pages, cu_seqlens, tok_pos, page_table, q_stride, table_width, num_pages, tokens, seqs, heads,
                           kv_heads, shared_pages, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks,
                           scale * 1.44269504088896341f};
     const hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)items, kv_heads), join(heads, tokens);
-#define SH_LAUNCH(DH)                                                             \
-    do {                                                                          \
-        if (items) attn_shared_kernel<DH><<<grid, SH_WAVES * 64, 0, s>>>(a);      \
-        attn_shared_join_kernel<DH><<<join, DH, 0, s>>>((bf16_t*)out, a);         \
+    const unsigned grid = (unsigned)items;
+    const dim3 join(heads, tokens);
+#define SH_LAUNCH(DH)                                                                        \
+    do {                                                                                     \
+        if (items == 0) {                                                                    \
+        } else if (p.nt == 0) attn_shared_kernel<DH, 0><<<grid, SH_WAVES * 64, 0, s>>>(a);   \
+        else if (p.nt == 1) attn_shared_kernel<DH, 1><<<grid, SH_WAVES * 64, 0, s>>>(a);     \
+        else attn_shared_kernel<DH, 2><<<grid, SH_WAVES * 64, 0, s>>>(a);                    \
+        attn_shared_join_kernel<DH><<<join, DH, 0, s>>>((bf16_t*)out, a);                    \
     } while (0)
     if (head_dim == 128) SH_LAUNCH(128);
     else if (head_dim == 64) SH_LAUNCH(64);

@@ -226,7 +226,9 @@ SHARED = [  # lens, shared, heads, kv, dim
     ([(1, 1)], 32, 2, 1, 32), ([(1, 33), (1, 5)], 64, 4, 2, 64), ([(1, 31), (1, 32), (1, 64)], 96, 8, 2, 128),
     ([(1, 40)] * 5, 0, 4, 4, 64), ([(3, 3), (1, 70), (5, 20), (2, 2)], 160, 6, 2, 64), ([(7, 30), (7, 7)], 32, 5, 1, 128),
     ([(1, 600), (1, 512), (1, 513), (2, 1025)], 32, 2, 2, 32), ([(4, 9)], 640, 3, 3, 128), ([(1, 3)] * 20, 288, 4, 1, 64),
-    ([(2, 500), (0, 33), (1, 1)], 512, 8, 1, 128), ([(1, 2)] * 70, 64, 1, 1, 32), ([(40, 40), (9, 100)], 64, 4, 2, 64),
+    # (from 33 columns of a key head on the pages go through LDS, tiles of 64 and, from 65 on, 128; an odd last page, one pair, one page)
+    ([(1, 2)] * 5, 288, 8, 1, 128), ([(2, 3)] * 5, 96, 8, 1, 128), ([(1, 1)] * 6, 32, 6, 1, 64), ([(3, 5)] * 15, 608, 3, 1, 32),
+    ([(1, 4)] * 17, 544, 16, 2, 64), ([(2, 500), (0, 33), (1, 1)], 512, 8, 1, 128), ([(1, 2)] * 70, 64, 1, 1, 32), ([(40, 40), (9, 100)], 64, 4, 2, 64),
 ]
 
 
@@ -249,6 +251,10 @@ def test_attention_over_shared_pages_of_tokens_within_them(ops):
     c = SharedCase([(1, 5), (2, 40)], 96, 4, 2, 64, seed=4)
     c.pos = [50, 95, 96 + 39]
     c.check(c.run(ops))
+    for heads in (12, 24):                                    # columns of a key head: 36 and 72
+        c = SharedCase([(1, 5), (2, 40)], 224, heads, 1, 32, seed=4)
+        c.pos = [70, 191, 224 + 39]
+        c.check(c.run(ops))
 
 
 def test_attention_over_shared_pages_finds_one_far_key(ops):
