@@ -15,7 +15,6 @@
 // infinity or NaN there reaches nothing.
 #include "attention_mfma.h"
 
-#define SH_WAVES 4
 #define SH_OWN_PAGES 16          // pages of a chunk of a sequence's own keys
 
 struct SharedArgs {
@@ -51,12 +50,13 @@ __device__ __forceinline__ void drop_behind(PageFrags<DH>& f, int last, int lane
     }
 }
 
-template <int DH>
+// W: wavefronts of a workgroup; SLOTS: pairs of pages of keys, and of values, that LDS holds (0: none, few columns only).
+template <int DH, int W, int SLOTS>
 struct SharedLds {
     static constexpr int LD = DH + 4;                        // a column's stride, floats
     union {
-        struct { bf16_t k[PAIR_SLOTS][2][PAGE * DH], v[PAIR_SLOTS][2][PAGE * DH]; } pages;
-        struct { float o[SH_WAVES][16 * LD], m[SH_WAVES][16], l[SH_WAVES][16]; } meet;
+        struct { bf16_t k[SLOTS ? SLOTS : 1][2][SLOTS ? PAGE * DH : 1], v[SLOTS ? SLOTS : 1][2][SLOTS ? PAGE * DH : 1]; } pages;
+        struct { float o[W][16 * LD], m[W][16], l[W][16]; } meet;
     };
 };
 
@@ -72,10 +72,10 @@ __device__ __forceinline__ size_t result_at(const SharedArgs& a, int slot, Place
 
 // Few columns: a tile of 16 over the pages page0 .. page1, which the wavefronts take in turn, each the next page on its way while it
 // weighs one; they meet in LDS.
-template <int DH>
-__device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& lds, const int32_t* table, int kvh, int slot,
+template <int DH, int W, int SLOTS>
+__device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, const int32_t* table, int kvh, int slot,
                                             int first_token, int col0, int cols, int page0, int page1, int last_key) {
-    constexpr int LD = SharedLds<DH>::LD;
+    constexpr int LD = SharedLds<DH, W, SLOTS>::LD;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
     Columns<DH, 1> c;
     init_columns<DH, 1>(c);
@@ -98,13 +98,13 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& 
     int page = page0 + wave;
     if (page < page1) {
         load(even, page);
-        for (;; page += 2 * SH_WAVES) {
-            load(odd, page + SH_WAVES);
+        for (;; page += 2 * W) {
+            load(odd, page + W);
             take(even, page);
-            if (page + SH_WAVES >= page1) break;
-            load(even, page + 2 * SH_WAVES);
-            take(odd, page + SH_WAVES);
-            if (page + 2 * SH_WAVES >= page1) break;
+            if (page + W >= page1) break;
+            load(even, page + 2 * W);
+            take(odd, page + W);
+            if (page + 2 * W >= page1) break;
         }
     }
     finish_columns<DH, 1>(c);
@@ -116,10 +116,10 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& 
     __syncthreads();
     float m = meet.m[0][i], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < SH_WAVES; ++w) m = fmaxf(m, meet.m[w][i]);
+    for (int w = 1; w < W; ++w) m = fmaxf(m, meet.m[w][i]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < SH_WAVES; ++w) l += __builtin_amdgcn_exp2f(meet.m[w][i] - ref) * meet.l[w][i];
+    for (int w = 0; w < W; ++w) l += __builtin_amdgcn_exp2f(meet.m[w][i] - ref) * meet.l[w][i];
     const float mine = __builtin_amdgcn_exp2f(c.m[0] - ref);
 #pragma unroll
     for (int dt = 0; dt < DH / 16; ++dt)
@@ -127,12 +127,12 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& 
             make_float4(c.o[0][dt][0] * mine, c.o[0][dt][1] * mine, c.o[0][dt][2] * mine, c.o[0][dt][3] * mine);
     if (wave == 0 && jg == 0 && col < cols) a.stats[result_at(a, slot, place)] = make_float2(m, l);
     __syncthreads();
-    for (int at = threadIdx.x; at < 16 * DH / 4; at += SH_WAVES * 64) {
+    for (int at = threadIdx.x; at < 16 * DH / 4; at += W * 64) {
         const int r = at / (DH / 4), d = at % (DH / 4) * 4;
         if (col0 + r >= cols) break;
         float4 o = *reinterpret_cast<const float4*>(&meet.o[0][r * LD + d]);
 #pragma unroll
-        for (int w = 1; w < SH_WAVES; ++w) {
+        for (int w = 1; w < W; ++w) {
             const float4 more = *reinterpret_cast<const float4*>(&meet.o[w][r * LD + d]);
             o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
         }
@@ -141,11 +141,13 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH>& 
 }
 
 // Many columns: a wavefront takes 16 NT of them and walks all pages page0 .. page1, two at a time (a pair that ends behind page1 takes
-// its last page twice, the second time masked); the pages are copied into LDS once for the four wavefronts, keys of pair u + 2 and values of
-// pair u + 1 while pair u is weighed, one place a turn where the wavefronts meet.
-template <int DH, int NT>
-__device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>& lds, int kvh, int slot, int col0, int cols, int page0, int page1) {
+// its last page twice, the second time masked); the pages are copied into LDS once for all wavefronts, one place a turn where they
+// meet.  A turn weighs pair u and takes the scores of pair u + 1; the copies of keys of pair u + SLOTS and values of pair
+// u + SLOTS - 1 start in it, so SLOTS - 1 turns hide a copy's way from memory.
+template <int DH, int NT, int W, int SLOTS>
+__device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, int kvh, int slot, int col0, int cols, int page0, int page1) {
     typedef CopiedPage<DH> Copied;
+    constexpr int HALVES = 8 / W, MINE = HALVES * Copied::MINE;         // half pages, and copies, of a wavefront for a pair
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
     const int last_key = page1 * PAGE - 1, u_last = (page1 - page0 - 1) / 2;
     auto& k_lds = lds.pages.k;
@@ -166,31 +168,36 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>&
     const bool all_seen = !__any(min_qpos < last_key);
     auto page_of = [&](int u) { return page0 + 2 * u; };
     auto open = [&](int u) { return all_seen && page_of(u) + 1 < page1; };
-    auto look = [&](int u, int h) -> int {
-        const int phys = a.page_table[min(page_of(min(u, u_last)) + h, page1 - 1)];
-        return min(max(phys, 0), a.num_pages - 1);
-    };
+    // The first half of the wavefronts copies keys, the other values: the same halves of one page, or of both, in every turn.
+    const bool of_values = wave >= W / 2;
     uint32_t off[Copied::MINE];
-    Copied::offsets(off, wave, lane);
-    auto fetch_keys = [&](int u, const int (&at)[2]) {       // (wavefronts 0 and 1)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-            Copied::copy(ma_lds(k_lds[(unsigned)u % PAIR_SLOTS][h]), off, a.k_pages + ((long)at[h] * a.kv_heads + kvh) * (PAGE * DH), wave);
+    Copied::offsets(off, (of_values ? 2 : 0) + (wave & 1), lane);
+    const bf16_t* pages = of_values ? a.v_pages : a.k_pages;
+    // Where the pages lie: a lane holds the place of one of 64 neighbouring pages.  (A load a turn would be counted among the copies
+    // under way; this one is waited for where it is made, once in 32 turns.)
+    int ids = 0, held = -1;
+    auto look = [&](int u, int n) -> int {                   // of the n-th page that this wavefront copies of pair u (behind the last: of it)
+        const int at = min(2 * min(u, u_last) + (HALVES == 2 ? n : wave >> 1 & 1), page1 - page0 - 1);
+        if (at >> 6 != held) {
+            held = at >> 6;
+            ids = a.page_table[min(page0 + 64 * held + lane, page1 - 1)];
+            ma_here(ids);
+        }
+        return min(max(__builtin_amdgcn_readlane(ids, at & 63), 0), a.num_pages - 1);
     };
-    auto fetch_values = [&](int u, const int (&at)[2]) {     // (wavefronts 2 and 3)
+    auto fetch = [&](int u, const int (&at)[HALVES]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            Copied::copy(ma_lds(v_lds[(unsigned)u % PAIR_SLOTS][h]), off, a.v_pages + ((long)at[h] * a.kv_heads + kvh) * (PAGE * DH), wave - 2);
-    };
-    auto fetch = [&](int u, const int (&k)[2], const int (&v)[2]) {       // keys of pair u, values of pair u - 1
-        if (wave < 2) fetch_keys(u, k);
-        else fetch_values(u - 1, v);
+        for (int n = 0; n < HALVES; ++n) {
+            const int h = HALVES == 2 ? n : wave >> 1 & 1;
+            const ma_lds_t to = of_values ? ma_lds(v_lds[(unsigned)u % SLOTS][h]) : ma_lds(k_lds[(unsigned)u % SLOTS][h]);
+            Copied::copy(to, off, pages + ((long)at[n] * a.kv_heads + kvh) * (PAGE * DH), wave & 1);
+        }
     };
     auto scores = [&](float (&s)[NT][2][8], int u) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             Frag kf[2][DH / 32];
-            Copied::keys(kf, k_lds[(unsigned)u % PAIR_SLOTS][h], lane);
+            Copied::keys(kf, k_lds[(unsigned)u % SLOTS][h], lane);
             float one[NT][8];
             scores_of<DH, NT>(c, kf, one, 0, lane);
 #pragma unroll
@@ -216,18 +223,16 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>&
         }
     };
     float s_cur[NT][2][8], ref[NT], m_new[NT];
-    int now[2], next[2];                                     // where the pages of pairs u + 1 and u + 2 lie
-    {
-        const int first[2] = {look(0, 0), look(0, 1)};
+    const int ahead = of_values ? SLOTS - 1 : SLOTS;         // turn u starts the copies of pair u + ahead
+    int next[HALVES];
+    for (int u = 0; u < ahead; ++u) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            now[h] = look(1, h);
-            next[h] = look(2, h);
-        }
-        if (wave < 2) fetch_keys(0, first);
-        fetch(1, now, first);
+        for (int n = 0; n < HALVES; ++n) next[n] = look(u, n);
+        fetch(u, next);
     }
-    ma_wait_copies<2 * Copied::MINE>();
+#pragma unroll
+    for (int n = 0; n < HALVES; ++n) next[n] = look(ahead, n);
+    ma_wait_copies<(SLOTS - 1) * MINE>();                     // the keys of pair 0 are there (the values: as many copies, one pair less)
     ma_meet();
     scores(s_cur, 0);
     if (!open(0)) mask(s_cur, 0);
@@ -243,19 +248,16 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>&
     };
     auto values = [&](const Frag (&w)[NT], int u, int h) {
         Frag vf[DH / 16];
-        Copied::values(vf, v_lds[(unsigned)u % PAIR_SLOTS][h], lane);
+        Copied::values(vf, v_lds[(unsigned)u % SLOTS][h], lane);
         weighted_values<DH, NT>(c, vf, w);
     };
     auto turn = [&](int u, auto masked) {                    // u: the pair whose weights are due
-        ma_wait_copies<0>();                                  // the keys of pair u + 1 and the values of pair u are there,
+        ma_wait_copies<(SLOTS - 2) * MINE>();                 // the keys of pair u + 1 and the values of pair u are there,
         ma_wait_lds();                                        // the keys of pair u and the values of pair u - 1 read
         ma_meet();
-        fetch(u + 2, next, now);
+        fetch(u + ahead, next);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            now[h] = next[h];
-            next[h] = look(u + 3, h);
-        }
+        for (int n = 0; n < HALVES; ++n) next[n] = look(u + ahead + 1, n);
         Frag w[2][NT];
         float s_next[NT][2][8];
         scores(s_next, u + 1);
@@ -298,9 +300,9 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH>&
 // NT: tiles of 16 columns a wavefront takes of the shared pages; 0: the wavefronts of a workgroup share one tile.
 // Workgroups by rising number: the shared pages' runs, a tile after the other, so that the tiles that read the same pages lie
 // a multiple of eight apart and meet in one XCD's L2; then the sequences' own chunks.
-template <int DH, int NT>
-__global__ void __launch_bounds__(SH_WAVES * 64, 2) attn_shared_kernel(const SharedArgs a) {
-    __shared__ __attribute__((aligned(16))) SharedLds<DH> lds;
+template <int DH, int NT, int W, int SLOTS>
+__global__ void __launch_bounds__(W * 64, 2) attn_shared_kernel(const SharedArgs a) {
+    __shared__ __attribute__((aligned(16))) SharedLds<DH, W, SLOTS> lds;
     const int of_tile = a.splits * a.kv_heads, shared_items = of_tile * a.tiles;
     int item = blockIdx.x;
     if (item < shared_items) {
@@ -309,8 +311,8 @@ __global__ void __launch_bounds__(SH_WAVES * 64, 2) attn_shared_kernel(const Sha
         const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads;
         const int page0 = slot * a.pages_per_split, page1 = min(page0 + a.pages_per_split, a.shared_pages);
         const int cols = a.tokens * (a.heads / a.kv_heads);
-        if (NT == 0) few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, cols, page0, page1, a.shared_pages * PAGE - 1);
-        else many_columns<DH, NT == 0 ? 1 : NT>(a, lds, kvh, slot, tile * 64 * NT, cols, page0, page1);
+        if constexpr (NT == 0) few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, cols, page0, page1, a.shared_pages * PAGE - 1);
+        else many_columns<DH, NT>(a, lds, kvh, slot, tile * 16 * W * NT, cols, page0, page1);
         return;
     }
     item -= shared_items;
@@ -328,48 +330,75 @@ __global__ void __launch_bounds__(SH_WAVES * 64, 2) attn_shared_kernel(const Sha
     few_columns<DH>(a, lds, a.page_table + (size_t)seq * a.table_width, kvh, a.splits + chunk, first, tile * 16, cols, page0, page1, last_key);
 }
 
-// A token's runs and chunks joined, a workgroup a (head, token); tokens that are no sequence's get zeros.
+// A token's runs and chunks joined, a workgroup a (head, token): DH / 4 neighbouring threads read a run's sums of it, 1,024 / DH
+// such groups take the runs in turn and meet in LDS in their order.  Tokens that are no sequence's get zeros.
+#define SH_JOIN 256
 template <int DH>
-__global__ void __launch_bounds__(DH) attn_shared_join_kernel(bf16_t* __restrict__ out, const SharedArgs a) {
-    const int head = blockIdx.x, token = blockIdx.y, d = threadIdx.x;
+__global__ void __launch_bounds__(SH_JOIN) attn_shared_join_kernel(bf16_t* __restrict__ out, const SharedArgs a) {
+    constexpr int LANES = DH / 4, GROUPS = SH_JOIN / LANES;
+    __shared__ __attribute__((aligned(16))) float4 sums[SH_JOIN];
+    __shared__ float2 stats[GROUPS];
+    const int head = blockIdx.x, token = blockIdx.y, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const int first = a.cu_seqlens[0], behind = a.cu_seqlens[a.seqs];
-    bf16_t* to = out + ((size_t)token * a.heads + head) * DH + d;
+    uint2* to = reinterpret_cast<uint2*>(out + ((size_t)token * a.heads + head) * DH) + lane;
     if (token < first || token >= behind) {
-        *to = 0;
+        if (group == 0) *to = uint2{0u, 0u};
         return;
     }
     const int own = min(a.tok_pos[token], a.table_width * PAGE - 1) + 1 - a.shared_pages * PAGE;      // own keys that it sees
     const int chunks = own > 0 ? min((own + SH_OWN_PAGES * PAGE - 1) / (SH_OWN_PAGES * PAGE), a.own_chunks) : 0;
     const int slots = a.splits + chunks;
     const size_t at = (size_t)token * a.heads + head, step = (size_t)a.tokens * a.heads;
-    float m = -INFINITY;
-    for (int s = 0; s < slots; ++s) m = fmaxf(m, a.stats[s * step + at].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o = 0.f;
-    for (int s = 0; s < slots; ++s) {
+    // a group's runs, its own running maximum and sums
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = group; s < slots; s += GROUPS) {
         const float2 st = a.stats[s * step + at];
-        const float w = __builtin_amdgcn_exp2f(st.x - ref);
-        l += w * st.y;
-        o += w * a.sums[(s * step + at) * DH + d];
+        const float4 v = *reinterpret_cast<const float4*>(a.sums + (s * step + at) * DH + 4 * lane);
+        const float m_new = fmaxf(m, st.x), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float before = __builtin_amdgcn_exp2f(m - ref), now = __builtin_amdgcn_exp2f(st.x - ref);
+        l = l * before + st.y * now;
+        o = make_float4(o.x * before + v.x * now, o.y * before + v.y * now, o.z * before + v.z * now, o.w * before + v.w * now);
+        m = m_new;
     }
-    *to = f32_to_bf16(l > 0.f ? o / l : 0.f);
+    if (lane == 0) stats[group] = make_float2(m, l);
+    sums[threadIdx.x] = o;
+    __syncthreads();
+    if (group > 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) m = fmaxf(m, stats[g].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        const float w = __builtin_amdgcn_exp2f(stats[g].x - ref);
+        const float4 v = sums[g * LANES + lane];
+        l += w * stats[g].y;
+        o = make_float4(o.x + w * v.x, o.y + w * v.y, o.z + w * v.z, o.w + w * v.w);
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    *to = uint2{pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv)};
 }
 
-struct SharedPlan { int nt, splits, pages_per_split, tiles, own_tiles, own_chunks; };
+struct SharedPlan { int nt, waves, splits, pages_per_split, tiles, own_tiles, own_chunks; };
 
-// More than 32 columns a key head take the form of many columns (a tile of 64 or, from 65 columns on, 128 a workgroup).  Runs of
-// the shared pages: two workgroups a compute unit, eight pages a run at least.
+// More than 32 columns a key head take the form of many columns: workgroups of four wavefronts with a tile of 64 or, from 65 columns on,
+// 128, from 129 on of eight with 256.  Runs of the shared pages: eight wavefronts a compute unit, eight pages a run at least.
 static SharedPlan shared_plan(int tokens, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     SharedPlan p;
     const int group = heads / kv_heads;
     const long cols = (long)tokens * group;
     p.nt = cols <= 32 ? 0 : cols <= 64 ? 1 : 2;
-    const int of_wg = p.nt == 0 ? 16 : 64 * p.nt;
+    p.waves = cols <= 128 ? 4 : 8;
+    const int of_wg = p.nt == 0 ? 16 : 16 * p.waves * p.nt;
     p.tiles = (int)((cols + of_wg - 1) / of_wg);
     p.own_tiles = (int)(((long)max_new * group + 15) / 16);
     const int own = max_len - shared_pages * PAGE;
     p.own_chunks = own > 0 ? (own + SH_OWN_PAGES * PAGE - 1) / (SH_OWN_PAGES * PAGE) : 0;
-    long runs = 2L * ri_compute_units() / ((long)p.tiles * kv_heads);
+    long runs = (p.waves == 4 ? 2L : 1L) * ri_compute_units() / ((long)p.tiles * kv_heads);
     if (runs < 1) runs = 1;
     p.pages_per_split = (int)((shared_pages + runs - 1) / runs);
     p.pages_per_split += p.pages_per_split & 1;
@@ -402,7 +431,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
     const SharedPlan p = shared_plan(tokens, max_new, shared_pages, max_len, heads, kv_heads);
     const long items = ((long)p.splits * p.tiles + (long)p.own_chunks * p.own_tiles * seqs) * kv_heads;
-    RI_REQUIRE(items <= 0x7fffffff / (SH_WAVES * 64), "attention_shared: %ld workgroups exceed one launch", items);
+    RI_REQUIRE(items <= 0x7fffffff / 512, "attention_shared: %ld workgroups exceed one launch", items);
     const size_t rows = (size_t)(p.splits + p.own_chunks) * tokens * heads;
     const SharedArgs a = {(float*)workspace, (float2*)((float*)workspace + rows * head_dim), (const bf16_t*)q, (const bf16_t*)k_pages,
                           (const bf16_t*)v_pages, cu_seqlens, tok_pos, page_table, q_stride, table_width, num_pages, tokens, seqs, heads,
@@ -414,10 +443,11 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
 #define SH_LAUNCH(DH)                                                                        \
     do {                                                                                     \
         if (items == 0) {                                                                    \
-        } else if (p.nt == 0) attn_shared_kernel<DH, 0><<<grid, SH_WAVES * 64, 0, s>>>(a);   \
-        else if (p.nt == 1) attn_shared_kernel<DH, 1><<<grid, SH_WAVES * 64, 0, s>>>(a);     \
-        else attn_shared_kernel<DH, 2><<<grid, SH_WAVES * 64, 0, s>>>(a);                    \
-        attn_shared_join_kernel<DH><<<join, DH, 0, s>>>((bf16_t*)out, a);                    \
+        } else if (p.nt == 0) attn_shared_kernel<DH, 0, 4, 0><<<grid, 256, 0, s>>>(a);       \
+        else if (p.nt == 1) attn_shared_kernel<DH, 1, 4, 2><<<grid, 256, 0, s>>>(a);         \
+        else if (p.waves == 4) attn_shared_kernel<DH, 2, 4, 2><<<grid, 256, 0, s>>>(a);      \
+        else attn_shared_kernel<DH, 2, 8, 4><<<grid, 512, 0, s>>>(a);                        \
+        attn_shared_join_kernel<DH><<<join, SH_JOIN, 0, s>>>((bf16_t*)out, a);               \
     } while (0)
     if (head_dim == 128) SH_LAUNCH(128);
     else if (head_dim == 64) SH_LAUNCH(64);

@@ -68,6 +68,13 @@ __device__ __forceinline__ void ma_meet() {
 }
 #endif
 
+// A value that is to be there at this place: the compiler waits for its load here, not where it is used.
+__device__ __forceinline__ void ma_here(int& v) {
+#ifndef RI_EMULATED
+    asm volatile("" : "+v"(v));
+#endif
+}
+
 // A value that the compiler is not to know anything about (the same for the whole wavefront).
 __device__ __forceinline__ void ma_opaque(uint32_t& v) {
 #ifndef RI_EMULATED
