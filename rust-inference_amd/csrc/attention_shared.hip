@@ -15,7 +15,7 @@
 // infinity or NaN there reaches nothing.
 #include "attention_mfma.h"
 
-#define SH_OWN_PAGES 16          // pages of a chunk of a sequence's own keys
+#define SH_OWN_PAGES 16          // pages of a chunk of a sequence's own keys: this many, or half where that leaves compute units empty
 
 struct SharedArgs {
     float* sums;                 // [slots][tokens][heads][dim]
@@ -27,26 +27,30 @@ struct SharedArgs {
     const int32_t* tok_pos;
     const int32_t* page_table;
     int q_stride, table_width, num_pages, tokens, seqs, heads, kv_heads, shared_pages;
-    int splits, pages_per_split, tiles, own_tiles, own_chunks;
+    int splits, pages_per_split, tiles, own_tiles, own_chunks, own_pages;
     float scale_log2;
 };
 
-// Key rows and value columns behind the last key (counted from the page's first) as zeros.
+// Key rows, and value columns, behind the last key (counted from the page's first) as zeros.
 template <int DH>
-__device__ __forceinline__ void drop_behind(PageFrags<DH>& f, int last, int lane) {
-    const int i = lane & 15, jg = lane >> 4;
+__device__ __forceinline__ void drop_keys(Frag (&kf)[2][DH / 32], int last, int lane) {
+    const int i = lane & 15;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
         if ((i >> 2) * 8 + kt * 4 + (i & 3) > last) {
 #pragma unroll
-            for (int ks = 0; ks < DH / 32; ++ks) f.k[kt][ks].u = make_uint4(0, 0, 0, 0);
+            for (int ks = 0; ks < DH / 32; ++ks) kf[kt][ks].u = make_uint4(0, 0, 0, 0);
         }
+}
+template <int DH>
+__device__ __forceinline__ void drop_values(Frag (&vf)[DH / 16], int last, int lane) {
+    const int jg = lane >> 4;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int key = jg * 8 + 2 * e;
         const uint32_t mask = key > last ? 0u : key + 1 > last ? 0x0000FFFFu : 0xFFFFFFFFu;
 #pragma unroll
-        for (int dt = 0; dt < DH / 16; ++dt) f.v[dt].w[e] &= mask;
+        for (int dt = 0; dt < DH / 16; ++dt) vf[dt].w[e] &= mask;
     }
 }
 
@@ -70,11 +74,16 @@ __device__ __forceinline__ size_t result_at(const SharedArgs& a, int slot, Place
     return ((size_t)slot * a.tokens + p.token) * a.heads + p.head;
 }
 
-// Few columns: a tile of 16 over the pages page0 .. page1, which the wavefronts take in turn, each the next page on its way while it
-// weighs one; they meet in LDS.
+// Where the first 64 pages from page0 on that a wavefront takes lie, a lane each (behind the last page there may be: the last).
+template <int W>
+__device__ __forceinline__ int first_ids(const int32_t* table, int page0, int pages) {
+    return table[min(page0 + (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 63) * W, pages - 1)];
+}
+
+// Few columns: a tile of 16 over the pages page0 .. page1, which the wavefronts take in turn; they meet in LDS.
 template <int DH, int W, int SLOTS>
 __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, const int32_t* table, int kvh, int slot,
-                                            int first_token, int col0, int cols, int page0, int page1, int last_key) {
+                                            int first_token, int col0, int cols, int page0, int page1, int last_key, int ids) {
     constexpr int LD = SharedLds<DH, W, SLOTS>::LD;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
     Columns<DH, 1> c;
@@ -85,26 +94,56 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W
     const bf16_t* q = a.q + (size_t)place.token * a.q_stride + place.head * DH + jg * 8;
 #pragma unroll
     for (int ks = 0; ks < DH / 32; ++ks) c.q[0][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
-    auto load = [&](PageFrags<DH>& f, int page) {            // (behind the last page: a line of it)
-        const int p = min(page, page1 - 1);
-        load_page<DH>(f, a.k_pages, a.v_pages, min(max(table[p], 0), a.num_pages - 1), a.kv_heads, kvh, lane, page < page1);
+    // The next page's keys are asked for when this one's are used up, its values likewise: a page is on its way all the time.
+    // (Behind the last page: a line of it.)
+    Frag kf[2][DH / 32], vf[DH / 16];
+    // A lane holds the place of one of the wavefront's next 64 pages (the caller has the first 64): a load a page would stand behind
+    // the values in the queue.
+    int held = 0;
+    auto phys_of = [&](int page) -> long {
+        const int at = (page - page0) / W;
+        if (at >> 6 != held) {
+            held = at >> 6;
+            ids = table[min(page0 + wave + (64 * held + lane) * W, page1 - 1)];
+            ma_here(ids);
+        }
+        return min(max(__builtin_amdgcn_readlane(ids, at & 63), 0), a.num_pages - 1);
     };
-    auto take = [&](PageFrags<DH>& f, int page) {
-        const int last = last_key - page * PAGE;
-        if (last < PAGE - 1) drop_behind<DH>(f, last, lane);
-        process_page<DH, 1>(c, f, page, lane, a.scale_log2, !__any(c.qpos[0] < page * PAGE + PAGE - 1));
+    auto load_keys = [&](long phys, bool wanted) {
+        const int w = wanted ? 1 : 0, r = i * w, g = jg * w;
+        const bf16_t* from = a.k_pages + (phys * a.kv_heads + kvh) * (long)(PAGE * DH);
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int ks = 0; ks < DH / 32; ++ks)
+                // (not marked as read once: a load takes 64 bytes of each of 16 rows, the next one the other half of those lines; marked,
+                // 64 sequences' own keys took 47 us, so 39)
+                kf[kt][ks].u = *reinterpret_cast<const uint4*>(from + ((r >> 2) * 8 + (kt * 4 + (r & 3)) * w) * DH + (ks * 32) * w + g * 8);
     };
-    PageFrags<DH> even, odd;
+    auto load_values = [&](long phys, bool wanted) {
+        const int w = wanted ? 1 : 0, r = i * w, g = jg * w;
+        const bf16_t* from = a.v_pages + (phys * a.kv_heads + kvh) * (long)(PAGE * DH);
+#pragma unroll
+        for (int dt = 0; dt < DH / 16; ++dt) vf[dt].u = load_stream16(from + (dt * 16 * w + r) * PAGE + g * 8);
+    };
     int page = page0 + wave;
     if (page < page1) {
-        load(even, page);
-        for (;; page += 2 * W) {
-            load(odd, page + W);
-            take(even, page);
-            if (page + W >= page1) break;
-            load(even, page + 2 * W);
-            take(odd, page + W);
-            if (page + 2 * W >= page1) break;
+        {
+            const long phys = phys_of(page);
+            load_keys(phys, true);
+            load_values(phys, true);
+        }
+        for (; page < page1; page += W) {
+            const int last = last_key - page * PAGE;
+            const bool more = page + W < page1;
+            Frag p[1];
+            if (last < PAGE - 1) drop_keys<DH>(kf, last, lane);
+            scores_and_weights<DH, 1>(c, kf, p, page, lane, a.scale_log2, !__any(c.qpos[0] < page * PAGE + PAGE - 1));
+            const long next = phys_of(page + W);
+            load_keys(next, more);
+            if (last < PAGE - 1) drop_values<DH>(vf, last, lane);
+            weighted_values<DH, 1>(c, vf, p);
+            load_values(next, more);
         }
     }
     finish_columns<DH, 1>(c);
@@ -142,8 +181,7 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W
 
 // Many columns: a wavefront takes 16 NT of them and walks all pages page0 .. page1, two at a time (a pair that ends behind page1 takes
 // its last page twice, the second time masked); the pages are copied into LDS once for all wavefronts, one place a turn where they
-// meet.  A turn weighs pair u and takes the scores of pair u + 1; the copies of keys of pair u + SLOTS and values of pair
-// u + SLOTS - 1 start in it, so SLOTS - 1 turns hide a copy's way from memory.
+// meet.  SLOTS - 1 turns hide a copy's way from memory.
 template <int DH, int NT, int W, int SLOTS>
 __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, int kvh, int slot, int col0, int cols, int page0, int page1) {
     typedef CopiedPage<DH> Copied;
@@ -152,6 +190,7 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
     const int last_key = page1 * PAGE - 1, u_last = (page1 - page0 - 1) / 2;
     auto& k_lds = lds.pages.k;
     auto& v_lds = lds.pages.v;
+    int ids = a.page_table[min(page0 + lane, page1 - 1)];
     Columns<DH, NT> c;
     init_columns<DH, NT>(c);
     int min_qpos = last_key;
@@ -166,6 +205,13 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
         for (int ks = 0; ks < DH / 32; ++ks) c.q[j][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
     }
     const bool all_seen = !__any(min_qpos < last_key);
+    // the queries are here before the first copy starts: a wait for them behind it would be one for all copies
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int ks = 0; ks < DH / 32; ++ks)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ma_here(c.q[j][ks].w[e]);
     auto page_of = [&](int u) { return page0 + 2 * u; };
     auto open = [&](int u) { return all_seen && page_of(u) + 1 < page1; };
     // The first half of the wavefronts copies keys, the other values: the same halves of one page, or of both, in every turn.
@@ -175,7 +221,7 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
     const bf16_t* pages = of_values ? a.v_pages : a.k_pages;
     // Where the pages lie: a lane holds the place of one of 64 neighbouring pages.  (A load a turn would be counted among the copies
     // under way; this one is waited for where it is made, once in 32 turns.)
-    int ids = 0, held = -1;
+    int held = 0;
     auto look = [&](int u, int n) -> int {                   // of the n-th page that this wavefront copies of pair u (behind the last: of it)
         const int at = min(2 * min(u, u_last) + (HALVES == 2 ? n : wave >> 1 & 1), page1 - page0 - 1);
         if (at >> 6 != held) {
@@ -297,37 +343,54 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
     }
 }
 
-// NT: tiles of 16 columns a wavefront takes of the shared pages; 0: the wavefronts of a workgroup share one tile.
-// Workgroups by rising number: the shared pages' runs, a tile after the other, so that the tiles that read the same pages lie
-// a multiple of eight apart and meet in one XCD's L2; then the sequences' own chunks.
-template <int DH, int NT, int W, int SLOTS>
-__global__ void __launch_bounds__(W * 64, 2) attn_shared_kernel(const SharedArgs a) {
-    __shared__ __attribute__((aligned(16))) SharedLds<DH, W, SLOTS> lds;
-    const int of_tile = a.splits * a.kv_heads, shared_items = of_tile * a.tiles;
-    int item = blockIdx.x;
-    if (item < shared_items) {
-        const int tile = item / of_tile;
-        item -= tile * of_tile;
-        const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads;
-        const int page0 = slot * a.pages_per_split, page1 = min(page0 + a.pages_per_split, a.shared_pages);
-        const int cols = a.tokens * (a.heads / a.kv_heads);
-        if constexpr (NT == 0) few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, cols, page0, page1, a.shared_pages * PAGE - 1);
-        else many_columns<DH, NT>(a, lds, kvh, slot, tile * 16 * W * NT, cols, page0, page1);
-        return;
-    }
-    item -= shared_items;
+// A sequence's own chunk, by its number among all (key heads fastest, then tiles, chunks, sequences).
+template <int DH, int W>
+__device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 0>& lds, int item) {
     const int kvh = item % a.kv_heads;
     item /= a.kv_heads;
     const int seq = item / (a.own_tiles * a.own_chunks);
     item -= seq * a.own_tiles * a.own_chunks;
-    const int chunk = item / a.own_tiles, tile = item - chunk * a.own_tiles;
+    const int chunk = item / a.own_tiles, tile = item - chunk * a.own_tiles, page0 = a.shared_pages + chunk * a.own_pages;
+    const int32_t* table = a.page_table + (size_t)seq * a.table_width;
+    // (asked for before the sequence's length is known: the loads of a chunk are a chain, and most of its time its first)
+    const int ids = first_ids<W>(table, page0, a.table_width);
     const int first = min(max(a.cu_seqlens[seq], 0), a.tokens), behind = min(max(a.cu_seqlens[seq + 1], first), a.tokens);
     const int cols = (behind - first) * (a.heads / a.kv_heads);
     if (tile * 16 >= cols) return;
     const int last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
-    const int page0 = a.shared_pages + chunk * SH_OWN_PAGES, page1 = min(page0 + SH_OWN_PAGES, last_key / PAGE + 1);
+    const int page1 = min(page0 + a.own_pages, last_key / PAGE + 1);
     if (page0 >= page1) return;
-    few_columns<DH>(a, lds, a.page_table + (size_t)seq * a.table_width, kvh, a.splits + chunk, first, tile * 16, cols, page0, page1, last_key);
+    few_columns<DH>(a, lds, table, kvh, a.splits + chunk, first, tile * 16, cols, page0, page1, last_key, ids);
+}
+
+// Few columns in all: the runs of the shared pages and the sequences' own chunks, a workgroup each; with more (ALL false) the own
+// chunks alone.
+template <int DH, bool ALL, int W>
+__global__ void __launch_bounds__(W * 64, 3) attn_shared_few_kernel(const SharedArgs a) {
+    __shared__ __attribute__((aligned(16))) SharedLds<DH, W, 0> lds;
+    const int of_tile = a.splits * a.kv_heads, shared_items = ALL ? of_tile * a.tiles : 0;
+    int item = blockIdx.x;
+    if (item >= shared_items) {
+        own_chunk<DH>(a, lds, item - shared_items);
+        return;
+    }
+    const int tile = item / of_tile;
+    item -= tile * of_tile;
+    const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads, page0 = slot * a.pages_per_split;
+    few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, a.tokens * (a.heads / a.kv_heads), page0,
+                    min(page0 + a.pages_per_split, a.shared_pages), a.shared_pages * PAGE - 1,
+                    first_ids<W>(a.page_table, page0, a.shared_pages));
+}
+
+// The shared pages' runs for many columns; by rising number a tile after the other, so that tiles that read the same pages lie a multiple
+// of eight apart and meet in one XCD's L2.
+template <int DH, int NT, int W, int SLOTS>
+__global__ void __launch_bounds__(W * 64, 2) attn_shared_kernel(const SharedArgs a) {
+    __shared__ __attribute__((aligned(16))) SharedLds<DH, W, SLOTS> lds;
+    const int of_tile = a.splits * a.kv_heads, tile = blockIdx.x / of_tile, item = blockIdx.x - tile * of_tile;
+    const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads, page0 = slot * a.pages_per_split;
+    many_columns<DH, NT>(a, lds, kvh, slot, tile * 16 * W * NT, a.tokens * (a.heads / a.kv_heads), page0,
+                         min(page0 + a.pages_per_split, a.shared_pages));
 }
 
 // A token's runs and chunks joined, a workgroup a (head, token): DH / 4 neighbouring threads read a run's sums of it, 1,024 / DH
@@ -346,7 +409,7 @@ __global__ void __launch_bounds__(SH_JOIN) attn_shared_join_kernel(bf16_t* __res
         return;
     }
     const int own = min(a.tok_pos[token], a.table_width * PAGE - 1) + 1 - a.shared_pages * PAGE;      // own keys that it sees
-    const int chunks = own > 0 ? min((own + SH_OWN_PAGES * PAGE - 1) / (SH_OWN_PAGES * PAGE), a.own_chunks) : 0;
+    const int chunks = own > 0 ? min((own + a.own_pages * PAGE - 1) / (a.own_pages * PAGE), a.own_chunks) : 0;
     const int slots = a.splits + chunks;
     const size_t at = (size_t)token * a.heads + head, step = (size_t)a.tokens * a.heads;
     // a group's runs, its own running maximum and sums
@@ -383,33 +446,39 @@ __global__ void __launch_bounds__(SH_JOIN) attn_shared_join_kernel(bf16_t* __res
     *to = uint2{pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv)};
 }
 
-struct SharedPlan { int nt, waves, splits, pages_per_split, tiles, own_tiles, own_chunks; };
+struct SharedPlan { int nt, waves, splits, pages_per_split, tiles, own_tiles, own_chunks, own_pages; };
 
 // More than 32 columns a key head take the form of many columns: workgroups of four wavefronts with a tile of 64 or, from 65 columns on,
-// 128, from 129 on of eight with 256.  Runs of the shared pages: eight wavefronts a compute unit, eight pages a run at least.
-static SharedPlan shared_plan(int tokens, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
+// 128, two of them a compute unit; from 129 columns on, where a run is longer than SH_SHORT_PAGES, of eight with 256, whose copies
+// have three turns to arrive instead of one.  us with four : eight wavefronts: 32 sequences of 64 heads behind 131,072 tokens (runs of 128
+// pages) 237 : 215, 64 of 32 heads behind 8,192 (8 pages) 78 : 79, 52 tokens of 32 heads behind 4,096 (8 pages) 43 : 47.  Runs of the
+// shared pages: eight wavefronts a compute unit, eight pages a run at least.
+#define SH_SHORT_PAGES 16
+static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     SharedPlan p;
     const int group = heads / kv_heads;
     const long cols = (long)tokens * group;
     p.nt = cols <= 32 ? 0 : cols <= 64 ? 1 : 2;
-    p.waves = cols <= 128 ? 4 : 8;
-    const int of_wg = p.nt == 0 ? 16 : 16 * p.waves * p.nt;
-    p.tiles = (int)((cols + of_wg - 1) / of_wg);
     p.own_tiles = (int)(((long)max_new * group + 15) / 16);
     const int own = max_len - shared_pages * PAGE;
-    p.own_chunks = own > 0 ? (own + SH_OWN_PAGES * PAGE - 1) / (SH_OWN_PAGES * PAGE) : 0;
-    long runs = (p.waves == 4 ? 2L : 1L) * ri_compute_units() / ((long)p.tiles * kv_heads);
-    if (runs < 1) runs = 1;
-    p.pages_per_split = (int)((shared_pages + runs - 1) / runs);
-    p.pages_per_split += p.pages_per_split & 1;
-    if (p.pages_per_split < 8) p.pages_per_split = 8;
+    p.own_pages = (long)seqs * kv_heads * p.own_tiles <= ri_compute_units() ? SH_OWN_PAGES / 2 : SH_OWN_PAGES;      // (max_len changes no sum)
+    p.own_chunks = own > 0 ? (own + p.own_pages * PAGE - 1) / (p.own_pages * PAGE) : 0;
+    for (p.waves = cols <= 128 ? 4 : 8;; p.waves = 4) {
+        const int of_wg = p.nt == 0 ? 16 : 16 * p.waves * p.nt;
+        p.tiles = (int)((cols + of_wg - 1) / of_wg);
+        const long runs = (p.waves == 4 ? 2L : 1L) * ri_compute_units() / ((long)p.tiles * kv_heads);
+        p.pages_per_split = (int)((shared_pages + (runs < 1 ? 1 : runs) - 1) / (runs < 1 ? 1 : runs));
+        p.pages_per_split += p.pages_per_split & 1;
+        if (p.pages_per_split < 8) p.pages_per_split = 8;
+        if (p.waves == 4 || p.pages_per_split > SH_SHORT_PAGES) break;
+    }
     p.splits = (shared_pages + p.pages_per_split - 1) / p.pages_per_split;
     return p;
 }
 
 extern "C" int ri_attention_shared_slots(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     if (tokens < 1 || seqs < 1 || max_new < 1 || shared_pages < 0 || max_len < 1 || kv_heads < 1 || heads < kv_heads) return 0;
-    const SharedPlan p = shared_plan(tokens, max_new, shared_pages, max_len, heads, kv_heads);
+    const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
     return p.splits + p.own_chunks;
 }
 
@@ -429,25 +498,29 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE((long)table_width * PAGE < 0x7fffffff, "attention_shared: page table width %d", table_width);
     RI_REQUIRE(scale > 0.f, "attention_shared: scale %g is not positive", (double)scale);
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
-    const SharedPlan p = shared_plan(tokens, max_new, shared_pages, max_len, heads, kv_heads);
-    const long items = ((long)p.splits * p.tiles + (long)p.own_chunks * p.own_tiles * seqs) * kv_heads;
-    RI_REQUIRE(items <= 0x7fffffff / 512, "attention_shared: %ld workgroups exceed one launch", items);
+    const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
+    const long of_shared = (long)p.splits * p.tiles * kv_heads, of_own = (long)p.own_chunks * p.own_tiles * seqs * kv_heads;
+    RI_REQUIRE(of_shared + of_own <= 0x7fffffff / 512, "attention_shared: %ld workgroups exceed one launch", of_shared + of_own);
     const size_t rows = (size_t)(p.splits + p.own_chunks) * tokens * heads;
     const SharedArgs a = {(float*)workspace, (float2*)((float*)workspace + rows * head_dim), (const bf16_t*)q, (const bf16_t*)k_pages,
                           (const bf16_t*)v_pages, cu_seqlens, tok_pos, page_table, q_stride, table_width, num_pages, tokens, seqs, heads,
-                          kv_heads, shared_pages, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks,
+                          kv_heads, shared_pages, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks, p.own_pages,
                           scale * 1.44269504088896341f};
     const hipStream_t s = (hipStream_t)stream;
-    const unsigned grid = (unsigned)items;
+    const unsigned own = (unsigned)of_own, shared = (unsigned)of_shared;
     const dim3 join(heads, tokens);
-#define SH_LAUNCH(DH)                                                                        \
-    do {                                                                                     \
-        if (items == 0) {                                                                    \
-        } else if (p.nt == 0) attn_shared_kernel<DH, 0, 4, 0><<<grid, 256, 0, s>>>(a);       \
-        else if (p.nt == 1) attn_shared_kernel<DH, 1, 4, 2><<<grid, 256, 0, s>>>(a);         \
-        else if (p.waves == 4) attn_shared_kernel<DH, 2, 4, 2><<<grid, 256, 0, s>>>(a);      \
-        else attn_shared_kernel<DH, 2, 8, 4><<<grid, 512, 0, s>>>(a);                        \
-        attn_shared_join_kernel<DH><<<join, SH_JOIN, 0, s>>>((bf16_t*)out, a);               \
+#define SH_LAUNCH(DH)                                                                                   \
+    do {                                                                                                \
+        if (p.nt == 0) {                                                                                \
+            if (own + shared) attn_shared_few_kernel<DH, true, 4><<<own + shared, 256, 0, s>>>(a);         \
+        } else {                                                                                        \
+            if (own) attn_shared_few_kernel<DH, false, 4><<<own, 256, 0, s>>>(a);                          \
+            if (shared == 0) {                                                                          \
+            } else if (p.nt == 1) attn_shared_kernel<DH, 1, 4, 2><<<shared, 256, 0, s>>>(a);            \
+            else if (p.waves == 4) attn_shared_kernel<DH, 2, 4, 2><<<shared, 256, 0, s>>>(a);           \
+            else attn_shared_kernel<DH, 2, 8, 4><<<shared, 512, 0, s>>>(a);                             \
+        }                                                                                               \
+        attn_shared_join_kernel<DH><<<join, SH_JOIN, 0, s>>>((bf16_t*)out, a);                          \
     } while (0)
     if (head_dim == 128) SH_LAUNCH(128);
     else if (head_dim == 64) SH_LAUNCH(64);

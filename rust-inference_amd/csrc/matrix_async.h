@@ -69,7 +69,8 @@ __device__ __forceinline__ void ma_meet() {
 #endif
 
 // A value that is to be there at this place: the compiler waits for its load here, not where it is used.
-__device__ __forceinline__ void ma_here(int& v) {
+template <class T>
+__device__ __forceinline__ void ma_here(T& v) {
 #ifndef RI_EMULATED
     asm volatile("" : "+v"(v));
 #endif
