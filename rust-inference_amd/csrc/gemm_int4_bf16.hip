@@ -9,14 +9,20 @@
 //
 // A code c becomes a bfloat16 by three bits of arithmetic: 16.0 has a step of 1/8 in its last place, so 0x4180 | c << 3 is
 // 16 + c, exactly, and two codes that lie 16 bits apart in a word turn in one instruction pair (mask and or after a shift).
-// What that adds, (16 + z) sum x, goes out again with sums of x that the matrix cores make of the same operands against
-// ones; both sums are float32 and the groups are short, so a sum of 128 numbers of 16 to 31 costs the result some three bits
-// of float32's 24.  Two codes that neighbour in a word are four columns apart, so x's words are permuted alike.
+// What that adds, s (16 + z) sum x, goes out again: the sums of x are made of the same operands against ones, and their products
+// with s (16 + z) are a product in float32 over the groups, four of them in an instruction of the matrix cores, whose operand
+// order is the order in which the lanes hold what they have loaded of s and z.  All sums are float32; taking off what was added
+// costs the result some three of its 24 bits.  Two codes that neighbour in a word are four columns apart, so x's words are
+// permuted alike.
 //
-// The wavefronts of a workgroup share the K pieces in turn and meet in LDS, in order.  Rows of x beyond M repeat the last
-// one (a row of the product depends on its own row of x alone) and are not stored; columns beyond K are zeros of x.
+// The wavefronts of a workgroup share the K pieces in turn and meet in LDS, in order.  A piece's codes (and x, where the
+// registers hold it twice) are asked for while the piece before is worked on; a lane group of four loads the scales and zero points
+// of the next four groups it meets, a group each, and three lane swaps hand all four to everybody.  Rows of x beyond M
+// repeat the last one (a row of the product depends on its own row of x alone) and are not stored; columns beyond K are zeros
+// of x.
 #include "api.h"
 #include "common.h"
+#include "matrix_async.h"
 
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 i4_bf16x8;
 typedef __attribute__((__vector_size__(4 * sizeof(float)))) float i4_floatx4;
@@ -29,6 +35,8 @@ union I4Frag {
 
 #define I4_PIECE 128             // columns a wavefront takes at a time: 16 bytes of codes a lane
 #define I4_ROWS 64               // rows of x a workgroup takes at most
+#define I4_NARROW 2              // tiles of 16 matrix rows a compute unit up to which a workgroup takes one of them
+#define I4_WIDE 12               // and up to which two (with up to 16 rows of x; then four)
 
 struct I4Args {
     void* out;
@@ -40,18 +48,39 @@ struct I4Args {
     int out_f32;
 };
 
-// Sixteen bytes from an address that is a multiple of four.
+// What a matrix without zero points reads in their place.
+static __device__ uint8_t i4_zero_point[4] = {8, 8, 8, 8};
+
+// Sixteen bytes from an address that is a multiple of four.  ONCE: marked as read once, for loads that take whole lines (a half line
+// marked so is fetched again for the other half).
+template <bool ONCE>
 __device__ __forceinline__ uint4 load16_by4(const uint8_t* p) {
     typedef unsigned int u32x4_t __attribute__((ext_vector_type(4), aligned(4)));
-    const u32x4_t v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p));
+    const u32x4_t* at = reinterpret_cast<const u32x4_t*>(p);
+    const u32x4_t v = ONCE ? __builtin_nontemporal_load(at) : *at;
     return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-// Word w of lane group s and word s of lane group w change places.
+// The words that the four lanes of a row hold, 8 columns each, brought to where a step's 32 columns are those of few groups.
+// STEPS 1: word s of lane group j has columns 32 s + 8 j .. +7; 2: those of 64 (s / 2) ..+63 in steps 2 (s / 2) and + 1; 4: as loaded.
+// column_of: the first of the eight.
+template <int STEPS>
+__device__ __forceinline__ int column_of(int s, int j) {
+    return STEPS == 1 ? 32 * s + 8 * j : STEPS == 2 ? 64 * (s >> 1) + 32 * (j & 1) + 16 * (j >> 1) + 8 * (s & 1) : 32 * j + 8 * s;
+}
+template <int STEPS>
 __device__ __forceinline__ void turn_words(uint32_t (&w)[4]) {
     typedef unsigned __attribute__((ext_vector_type(2))) pair_t;
+    if (STEPS == 4) return;
     const pair_t a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
     const pair_t b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    if (STEPS == 2) {
+        w[0] = a.x;
+        w[1] = b.x;
+        w[2] = a.y;
+        w[3] = b.y;
+        return;
+    }
     const pair_t c = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false);
     const pair_t d = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
     w[0] = c.x;
@@ -60,12 +89,14 @@ __device__ __forceinline__ void turn_words(uint32_t (&w)[4]) {
     w[3] = d.y;
 }
 
-// Eight codes as 16 + c, in the order 0 4 1 5 2 6 3 7 of the word's nibbles.
-__device__ __forceinline__ void widen(I4Frag& f, uint32_t w) {
-    f.w[0] = ((w << 3) & 0x00780078u) | 0x41804180u;
-    f.w[1] = ((w >> 1) & 0x00780078u) | 0x41804180u;
-    f.w[2] = ((w >> 5) & 0x00780078u) | 0x41804180u;
-    f.w[3] = ((w >> 9) & 0x00780078u) | 0x41804180u;
+// Eight codes as 16 + c, in the order 0 4 1 5 2 6 3 7 of the word's nibbles.  mask is 0x00780078 and sixteen 0x41804180, held in
+// registers that the compiler does not see through: an instruction takes one literal, and with two the and and the or would be
+// one each.
+__device__ __forceinline__ void widen(I4Frag& f, uint32_t w, uint32_t mask, uint32_t sixteen) {
+    f.w[0] = ((w << 3) & mask) | sixteen;
+    f.w[1] = ((w >> 1) & mask) | sixteen;
+    f.w[2] = ((w >> 5) & mask) | sixteen;
+    f.w[3] = ((w >> 9) & mask) | sixteen;
 }
 // Eight neighbouring numbers in the same order.
 __device__ __forceinline__ void reorder(I4Frag& f, const uint4 u) {
@@ -75,93 +106,182 @@ __device__ __forceinline__ void reorder(I4Frag& f, const uint4 u) {
     f.w[3] = __builtin_amdgcn_perm(u.w, u.y, 0x07060302u);
 }
 
-__device__ __forceinline__ float scale_at(const float* s, size_t i) { return s[i]; }
-__device__ __forceinline__ float scale_at(const bf16_t* s, size_t i) { return bf16_to_f32(s[i]); }
+// acc += a . b of the matrix cores' 16 x 16 x 4 product in float32: lane l holds a[l % 16][l / 16] and b[l / 16][l % 16].
+__device__ __forceinline__ void add_product4(i4_floatx4& acc, float a, float b) { acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); }
+
+// sum over the 32 STEPS columns of x's fragments from xf on, of row l % 16 in lane l.
+template <int STEPS>
+__device__ __forceinline__ float sum_of(const I4Frag* xf, const I4Frag& ones) {
+    i4_floatx4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones.v, xf[i].v, s, 0, 0, 0);
+    return s[0];
+}
+
+// A lane group's value in every one of the four.
+__device__ __forceinline__ void to_all(float (&all)[4], float v) {
+    typedef unsigned __attribute__((ext_vector_type(2))) pair_t;
+    const unsigned u = __float_as_uint(v);
+    const pair_t a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const pair_t low = __builtin_amdgcn_permlane16_swap(a.x, a.x, false, false), high = __builtin_amdgcn_permlane16_swap(a.y, a.y, false, false);
+    const unsigned r0 = low.x, r1 = low.y, r2 = high.x, r3 = high.y;
+    all[0] = __uint_as_float(r0);
+    all[1] = __uint_as_float(r1);
+    all[2] = __uint_as_float(r2);
+    all[3] = __uint_as_float(r3);
+}
 
 // MT tiles of 16 rows of x, NT tiles of 16 rows of the matrix, W wavefronts.  STEPS: steps of 32 columns that share a group
 // (4: groups are multiples of 128).
 template <int MT, int NT, int W, int STEPS, typename S>
 __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) {
-    const int lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE, i = lane & 15, j = lane >> 4;
+    constexpr int USES = 4 / STEPS, ROUND = STEPS;            // groups that a piece meets; pieces that meet four groups
+    constexpr int TURN = ROUND < 2 ? 2 : ROUND;               // pieces a turn of the loop: an even number, two buffers
+    constexpr bool X_TWICE = MT <= 2;
+    const int lane = threadIdx.x & (RI_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / RI_WAVE), i = lane & 15, j = lane >> 4;
     const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * I4_ROWS;
-    const int pieces = (a.k + I4_PIECE - 1) / I4_PIECE;
+    const int full = a.k / I4_PIECE, pieces = (a.k + I4_PIECE - 1) / I4_PIECE;
     const size_t row_bytes = (size_t)a.k / 2;
     const S* scales = (const S*)a.scales;
-    int col[NT];
+    const uint8_t* zeros = a.zeros ? a.zeros : i4_zero_point;
+    const int zero_step = a.zeros ? 1 : 0;
     const uint8_t* code_row[NT];
+    size_t group_row[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        col[t] = min(n0 + 16 * t + i, a.n - 1);
-        code_row[t] = a.codes + col[t] * row_bytes;
+        const size_t col = min(n0 + 16 * t + i, a.n - 1);
+        code_row[t] = a.codes + col * row_bytes + 16 * j;
+        group_row[t] = col * a.groups;
     }
     const bf16_t* x_row[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) x_row[t] = a.x + (size_t)min(m0 + 16 * t + i, a.rows - 1) * a.k;
+    for (int t = 0; t < MT; ++t) x_row[t] = a.x + (size_t)min(m0 + 16 * t + i, a.rows - 1) * a.k + 8 * j;
 
     i4_floatx4 total[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int t = 0; t < NT; ++t) total[mt][t] = i4_floatx4{0.f, 0.f, 0.f, 0.f};
+    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
+    ma_opaque(mask);
+    ma_here(sixteen);
     I4Frag ones;
     ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = 0x3F803F80u;
 
-    for (int p = wave; p < pieces; p += W) {
-        const int k0 = p * I4_PIECE;
-        uint32_t w[NT][4];
-        if (k0 + I4_PIECE <= a.k) {
+    struct Groups { S scale[NT]; uint8_t zero[NT]; };        // as loaded: a conversion would wait for the load
+    // Loads stay out of branches, so that the compiler counts them in flight: one that nobody wants reads what every lane reads.
+    auto load_codes = [&](uint4 (&c)[NT], int p, bool wanted) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const uint4 u = load16_by4(code_row[t] + k0 / 2 + 16 * j);
-                w[t][0] = u.x, w[t][1] = u.y, w[t][2] = u.z, w[t][3] = u.w;
-            }
-        } else {                                              // the row ends within the piece
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    w[t][q] = *reinterpret_cast<const uint32_t*>(code_row[t] + min((size_t)(k0 / 2 + 16 * j + 4 * q), row_bytes - 4));
-        }
-        I4Frag xf[MT][4];
+        for (int t = 0; t < NT; ++t) c[t] = load16_by4<false>(wanted ? code_row[t] + p * (I4_PIECE / 2) : a.codes);
+    };
+    auto load_x = [&](uint4 (&x)[MT][4], int p, bool wanted) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = k0 + 32 * s + 8 * j;
-                const uint4 u = *reinterpret_cast<const uint4*>(k < a.k ? x_row[mt] + k : ri_zero_fragment + 8 * lane);
-                reorder(xf[mt][s], u);
+            for (int s = 0; s < 4; ++s) x[mt][s] = *reinterpret_cast<const uint4*>(wanted ? x_row[mt] + p * I4_PIECE + 32 * s : a.x);
+    };
+    // The four groups that the wavefront meets from piece p on, group e of them by lane group e.
+    auto load_groups = [&](Groups& g, int p) {
+        const int piece = min(p + (j / USES) * W, pieces - 1);
+        const int group = STEPS == 4 ? (a.per == 1 ? piece : piece / a.per) : min(piece * USES + j % USES, a.groups - 1);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            g.scale[t] = scales[group_row[t] + group];
+            g.zero[t] = zeros[(group_row[t] + group) * zero_step];
+        }
+    };
+    float scale[NT][4], less[NT];                            // of four groups: every lane all of them; lane group e of the e-th
+    auto spread = [&](const Groups& g) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float own = to_f32(g.scale[t]);
+            to_all(scale[t], own);
+            less[t] = -own * (16.f + (float)g.zero[t]);
+        }
+    };
+    // first: which of the four groups the piece meets first
+    auto work = [&](const uint4 (&codes)[NT], const uint4 (&x)[MT][4], int first) {
+        I4Frag xf[MT][4];
+        float sum[MT];                                        // of the group that lane group j holds, 0 where the piece has none such
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) reorder(xf[mt][s], x[mt][s]);
+            sum[mt] = 0.f;
+#pragma unroll
+            for (int e = 0; e < USES; ++e) {
+                const float one = sum_of<STEPS>(xf[mt] + e * STEPS, ones);
+                sum[mt] = j == first + e ? one : sum[mt];
             }
+        }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) turn_words(w[t]);
+        for (int t = 0; t < NT; ++t) {
+            uint32_t w[4] = {codes[t].x, codes[t].y, codes[t].z, codes[t].w};
+            turn_words<1>(w);
 #pragma unroll
-        for (int s0 = 0; s0 < 4; s0 += STEPS) {
-            const int group = STEPS == 4 ? (a.per == 1 ? p : p / a.per) : min((4 * p + s0) / STEPS, a.groups - 1);
-            i4_floatx4 sum[MT];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                sum[mt] = i4_floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = s0; s < s0 + STEPS; ++s)
-                    sum[mt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[mt][s].v, ones.v, sum[mt], 0, 0, 0);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const size_t at = (size_t)col[t] * a.groups + group;
-                const float scale = scale_at(scales, at), off = 16.f + (a.zeros ? (float)a.zeros[at] : 8.f);
+            for (int e = 0; e < USES; ++e) {
                 I4Frag wf[STEPS];
 #pragma unroll
-                for (int s = 0; s < STEPS; ++s) widen(wf[s], w[t][s0 + s]);
+                for (int s = 0; s < STEPS; ++s) widen(wf[s], w[e * STEPS + s], mask, sixteen);
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt) {
                     i4_floatx4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[mt][s0 + s].v, wf[s].v, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[mt][e * STEPS + s].v, wf[s].v, acc, 0, 0, 0);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) total[mt][t][e] = fmaf(scale, fmaf(-off, sum[mt][e], acc[e]), total[mt][t][e]);
+                    for (int q = 0; q < 4; ++q) total[mt][t][q] = fmaf(scale[t][first + e], acc[q], total[mt][t][q]);
                 }
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) add_product4(total[mt][t], sum[mt], less[t]);
         }
+    };
+
+    if (wave < full) {
+        uint4 codes[2][NT], x[X_TWICE ? 2 : 1][MT][4];
+        Groups g;
+        load_groups(g, wave);
+        if (X_TWICE) load_x(x[0], wave, true);
+        load_codes(codes[0], wave, true);
+        for (int p = wave;; p += TURN * W) {
+#pragma unroll
+            for (int q = 0; q < TURN; ++q) {
+                const int at = p + q * W;
+                const bool more = at + W < full;
+                if (q > 0 && at >= full) break;
+                if (q % ROUND == 0) {
+                    spread(g);
+                    load_groups(g, at + ROUND * W);
+                }
+                if (X_TWICE) load_x(x[X_TWICE ? (q + 1) % 2 : 0], at + W, more);
+                else load_x(x[0], at, true);
+                load_codes(codes[(q + 1) % 2], at + W, more);
+                work(codes[q % 2], x[X_TWICE ? q % 2 : 0], q % ROUND * USES);
+            }
+            if (p + TURN * W >= full) break;
+        }
+    }
+    if (pieces > full && full % W == wave) {                  // the row ends within the last piece
+        const int k0 = full * I4_PIECE;
+        uint4 codes[NT], x[MT][4];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)                       // (a word of eight codes is there whole or not at all)
+                w[q] = *reinterpret_cast<const uint32_t*>(code_row[t] - 16 * j + min((size_t)(k0 / 2 + 16 * j + 4 * q), row_bytes - 4));
+            codes[t] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                x[mt][s] = *reinterpret_cast<const uint4*>(k0 + 32 * s + 8 * j < a.k ? x_row[mt] + k0 + 32 * s : ri_zero_fragment + 8 * lane);
+        Groups g;
+        load_groups(g, full);
+        spread(g);
+        work(codes, x, 0);
     }
 
     // the wavefronts' sums, added in their order: lane l holds rows 4 j .. +3 of column i of every tile
@@ -203,6 +323,210 @@ __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) 
         }
 }
 
+// Of two neighbouring lanes: the even one's low in itself and its high in the odd one; the odd one's low in the even one and its high.
+__device__ __forceinline__ uint32_t neighbour(uint32_t v) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, false); }
+__device__ __forceinline__ uint32_t from_even(bool odd, uint32_t low, uint32_t high) {
+    const uint32_t other = neighbour(high);                   // (all lanes take part)
+    return odd ? other : low;
+}
+__device__ __forceinline__ uint32_t from_odd(bool odd, uint32_t low, uint32_t high) {
+    const uint32_t other = neighbour(low);
+    return odd ? high : other;
+}
+
+// Many matrix rows, up to 16 rows of x: a workgroup's eight wavefronts hold x for the whole of K, PP pieces each in the order of the
+// product and summed per group, and go from one tile of 16 matrix rows to the next; of a tile a wavefront reads its PP pieces, so
+// that the workgroup reads 16 whole rows, neighbours in memory.  AHEAD tiles' codes are on their way while one is worked on.  The
+// wavefronts' sums of eight tiles wait in LDS; then they meet, and each adds up and stores one tile (a place to meet for every
+// tile, and one wavefront there adding while the others wait at the next, took 88 us for 151,936 x 4,096).
+template <int PP, int AHEAD, int STEPS, typename S>
+__global__ __launch_bounds__(8 * RI_WAVE, 2) void gemm_int4_rows_kernel(const I4Args a) {
+    constexpr int W = 8, USES = 4 / STEPS, BLOCKS = (PP * USES + 3) / 4;       // groups that a piece meets; loads of four groups for the pieces
+    __shared__ __attribute__((aligned(16))) float4 meet[2][W][W][RI_WAVE];
+    const int lane = threadIdx.x & (RI_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / RI_WAVE), i = lane & 15, j = lane >> 4;
+    const int tiles = (a.n + 15) / 16, pieces = (a.k + I4_PIECE - 1) / I4_PIECE, first = wave * PP;
+    const size_t row_bytes = (size_t)a.k / 2;
+    const S* scales = (const S*)a.scales;
+    const uint8_t* zeros = a.zeros ? a.zeros : i4_zero_point;
+    const uint32_t zero_mask = a.zeros ? ~0u : 0u;
+
+    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
+    ma_opaque(mask);
+    ma_here(sixteen);
+    I4Frag ones, xf[PP][4];
+    float sum[BLOCKS];                                        // of the groups that lane group j holds
+    ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = 0x3F803F80u;
+    const bf16_t* x_row = a.x + (size_t)min(i, a.rows - 1) * a.k;
+#pragma unroll
+    for (int p = 0; p < PP; ++p)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int k = (first + p) * I4_PIECE + column_of<STEPS>(s, j);
+            xf[p][s].u = *reinterpret_cast<const uint4*>(k < a.k ? x_row + k : ri_zero_fragment + 8 * lane);
+        }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) sum[b] = 0.f;
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) reorder(xf[p][s], xf[p][s].u);
+#pragma unroll
+        for (int e = 0; e < USES; ++e) {
+            const float one = sum_of<STEPS>(xf[p] + e * STEPS, ones);
+            const int use = p * USES + e;
+            sum[use / 4] = j == use % 4 ? one : sum[use / 4];
+        }
+    }
+    // A load takes whole 128-byte lines of eight rows: of a pair of pieces lanes 2 r and 2 r + 1 of every sixteen ask for row r's 256 columns
+    // in one and for row 8 + r's in the other; then neighbours exchange, so that an even lane holds row r and an odd one row
+    // 8 + r, of the first piece and of the second.  (151,936 x 4,096: 79 us; with loads of half a line of sixteen rows, fewer
+    // instructions, 87.)  A lane's 32 columns are there whole or not at all: then the row's first, against zeros of x.
+    const bool odd = i & 1;
+    const int row_of = (i >> 1) + 8 * (i & 1);               // the row of a tile that a lane's column of the product is
+    uint32_t at[PP / 2], group[BLOCKS];
+#pragma unroll
+    for (int p = 0; p < PP / 2; ++p) {
+        const int k = (first + 2 * p) * I4_PIECE + 128 * (i & 1) + 32 * j;
+        at[p] = k < a.k ? k / 2 : 0;
+    }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        const int use = 4 * b + j, piece = min(first + min(use / USES, PP - 1), pieces - 1);
+        group[b] = STEPS == 4 ? (a.per == 1 ? piece : piece / a.per) : min(piece * USES + use % USES, a.groups - 1);
+    }
+    struct Tile { uint4 codes[PP]; S scale[BLOCKS]; uint8_t zero[BLOCKS]; };      // as loaded: a conversion would wait for the load
+    // The tiles follow one another at a fixed distance; rows behind the last are the last.  (Offsets of 32 bits, moved on, not made anew:
+    // what this loop does is bound by the instructions that it issues.)
+    const uint32_t last_row = (uint32_t)(a.n - 1) * (uint32_t)row_bytes, last_groups = (uint32_t)(a.n - 1) * (uint32_t)a.groups;
+    const uint32_t row_step = 16u * gridDim.x * (uint32_t)row_bytes, groups_step = 16u * gridDim.x * (uint32_t)a.groups;
+    auto row_at = [&](int r) { return (uint32_t)min(16 * (int)blockIdx.x + r, a.n - 1); };
+    uint32_t low = row_at(i >> 1) * (uint32_t)row_bytes, high = row_at(8 + (i >> 1)) * (uint32_t)row_bytes, groups = row_at(row_of) * (uint32_t)a.groups;
+    auto load = [&](Tile& t) {                                // the next tile's
+#pragma unroll
+        for (int p = 0; p < PP / 2; ++p) {
+            t.codes[2 * p] = load16_by4<true>(a.codes + (low + at[p]));
+            t.codes[2 * p + 1] = load16_by4<true>(a.codes + (high + at[p]));
+        }
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            const uint32_t g = groups + group[b];
+            t.scale[b] = *reinterpret_cast<const S*>(reinterpret_cast<const char*>(scales) + (uint32_t)(g * sizeof(S)));
+            t.zero[b] = zeros[g & zero_mask];
+        }
+        low = last_row - low < row_step ? last_row : low + row_step;
+        high = last_row - high < row_step ? last_row : high + row_step;
+        groups = last_groups - groups < groups_step ? last_groups : groups + groups_step;
+    };
+    auto work = [&](const Tile& t, int turn) {
+        i4_floatx4 total = {0.f, 0.f, 0.f, 0.f};
+        float scale[BLOCKS][4];
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) {
+            const float own = to_f32(t.scale[b]);
+            to_all(scale[b], own);
+            add_product4(total, sum[b], -own * (16.f + (float)t.zero[b]));
+        }
+        I4Frag wf[2][4];
+#pragma unroll
+        for (int p = 0; p < PP; ++p) {
+            const uint4 lo = t.codes[p & ~1], hi = t.codes[p | 1];
+            uint32_t w[4];
+            if (p % 2 == 0) {
+                w[0] = from_even(odd, lo.x, hi.x), w[1] = from_even(odd, lo.y, hi.y);
+                w[2] = from_even(odd, lo.z, hi.z), w[3] = from_even(odd, lo.w, hi.w);
+            } else {
+                w[0] = from_odd(odd, lo.x, hi.x), w[1] = from_odd(odd, lo.y, hi.y);
+                w[2] = from_odd(odd, lo.z, hi.z), w[3] = from_odd(odd, lo.w, hi.w);
+            }
+            turn_words<STEPS>(w);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) widen(wf[p % 2][s], w[s], mask, sixteen);
+            if (p % 2 == 0) continue;
+            // two pieces' products, none of which waits for another one's sum, then what they weigh
+            i4_floatx4 acc[2][USES];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < USES; ++e) acc[h][e] = i4_floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < USES; ++e)
+                        acc[h][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xf[p - 1 + h][e * STEPS + s].v, wf[h][e * STEPS + s].v, acc[h][e], 0, 0, 0);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < USES; ++e) {
+                    const int use = (p - 1 + h) * USES + e;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) total[q] = fmaf(scale[use / 4][use % 4], acc[h][e][q], total[q]);
+                }
+        }
+        meet[turn / W & 1][turn % W][wave][lane] = make_float4(total[0], total[1], total[2], total[3]);
+    };
+    auto store = [&](int tile, int turn) {                    // the tile of that turn, added up
+        const auto& from = meet[turn / W & 1][turn % W];
+        float4 o = from[0][lane];
+#pragma unroll
+        for (int v = 1; v < W; ++v) {
+            const float4 more = from[v][lane];
+            o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
+        }
+        const int col = 16 * tile + row_of;
+        const float value[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int m = 4 * j + e;
+            if (m < a.rows && col < a.n) {
+                if (a.out_f32) ((float*)a.out)[(size_t)m * a.n + col] = value[e];
+                else ((bf16_t*)a.out)[(size_t)m * a.n + col] = f32_to_bf16(value[e]);
+            }
+        }
+    };
+    const int step = gridDim.x;
+    Tile ring[AHEAD + 1];
+    int tile = blockIdx.x, turn = 0;
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+        load(ring[d]);
+        __builtin_amdgcn_sched_barrier(0);                    // (in this order: the loop's waits count by the order of entry too)
+    }
+    do {                                                      // (one way out: with one a tile the compiler waits for every load at the top)
+#pragma unroll
+        for (int d = 0; d <= AHEAD; ++d) {
+            load(ring[(d + AHEAD) % (AHEAD + 1)]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (tile < tiles) {
+                work(ring[d], turn);
+                if (turn % W == W - 1 || tile + step >= tiles) {
+                    __syncthreads();                          // (a buffer is written again behind the next such place)
+                    const int mine = turn / W * W + wave;
+                    if (mine <= turn) store(blockIdx.x + mine * step, mine);
+                }
+                ++turn;
+            }
+            tile += step;
+        }
+    } while (tile < tiles);
+}
+
+template <int PP, int AHEAD>
+static void int4_rows(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
+    const int tiles = (a.n + 15) / 16, rounds = (tiles + ri_compute_units() - 1) / ri_compute_units();
+    const unsigned grid = (tiles + rounds - 1) / rounds;      // (as many tiles a workgroup)
+#define I4_ROWS_LAUNCH(STEPS)                                                                                    \
+    do {                                                                                                         \
+        if (scale_f32) gemm_int4_rows_kernel<PP, AHEAD, STEPS, float><<<grid, 8 * RI_WAVE, 0, s>>>(a);           \
+        else gemm_int4_rows_kernel<PP, AHEAD, STEPS, bf16_t><<<grid, 8 * RI_WAVE, 0, s>>>(a);                    \
+    } while (0)
+    if (group == 32) I4_ROWS_LAUNCH(1);
+    else if (group == 64) I4_ROWS_LAUNCH(2);
+    else I4_ROWS_LAUNCH(4);
+#undef I4_ROWS_LAUNCH
+}
+
 template <int MT, int NT, int W, int STEPS>
 static void int4_launch(const I4Args& a, bool scale_f32, hipStream_t s) {
     const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.rows + I4_ROWS - 1) / I4_ROWS);
@@ -210,11 +534,19 @@ static void int4_launch(const I4Args& a, bool scale_f32, hipStream_t s) {
     else gemm_int4_kernel<MT, NT, W, STEPS, bf16_t><<<grid, W * RI_WAVE, 0, s>>>(a);
 }
 
-template <int MT>
+template <int MT, int NT, int W>
 static void int4_by_group(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
-    if (group == 32) int4_launch<MT, 1, 8, 1>(a, scale_f32, s);
-    else if (group == 64) int4_launch<MT, 1, 8, 2>(a, scale_f32, s);
-    else int4_launch<MT, 1, 8, 4>(a, scale_f32, s);
+    if (group == 32) int4_launch<MT, NT, W, 1>(a, scale_f32, s);
+    else if (group == 64) int4_launch<MT, NT, W, 2>(a, scale_f32, s);
+    else int4_launch<MT, NT, W, 4>(a, scale_f32, s);
+}
+
+template <int MT>
+static void int4_by_width(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
+    const int tiles = (a.n + 15) / 16, units = ri_compute_units();
+    if (tiles <= I4_NARROW * units) int4_by_group<MT, 1, 8>(a, group, scale_f32, s);
+    else if (MT > 1 || tiles <= I4_WIDE * units) int4_by_group<MT, 2, 4>(a, group, scale_f32, s);
+    else int4_by_group<MT, MT == 1 ? 4 : 2, 4>(a, group, scale_f32, s);
 }
 
 extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const void* codes, const void* scales, int scale_dtype,
@@ -233,11 +565,13 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
                       group >= 128 ? group / 128 : 1, out_dtype == RI_F32};
     const bool f = scale_dtype == RI_F32;
     const hipStream_t s = (hipStream_t)stream;
-    const int mt = rows >= I4_ROWS ? 4 : (rows + 15) / 16;
-    if (mt == 1) int4_by_group<1>(a, group, f, s);
-    else if (mt == 2) int4_by_group<2>(a, group, f, s);
-    else if (mt == 3) int4_by_group<3>(a, group, f, s);
-    else int4_by_group<4>(a, group, f, s);
+    const int pieces = (k + I4_PIECE - 1) / I4_PIECE;
+    if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && (n + 15) / 16 > I4_NARROW * ri_compute_units()) {
+        if (pieces <= 16) int4_rows<2, 2>(a, group, f, s);
+        else int4_rows<4, 1>(a, group, f, s);
+    } else if (rows <= 16) int4_by_width<1>(a, group, f, s);
+    else if (rows <= 32) int4_by_width<2>(a, group, f, s);
+    else int4_by_width<4>(a, group, f, s);
     RI_LAUNCH_CHECK("gemm_int4");
     return 0;
 }

@@ -18,9 +18,20 @@ def test_the_kernels_of_a_drafted_step_pass_on_the_cpu_build_between_guard_pages
         emulated.library()
     except KernelError as e:
         pytest.skip(f"no CPU build of the kernels here: {e}")
+    # (with one compute unit the products of many matrix rows and the runs of many pages are chosen at these sizes)
+    for units, select in (("", ""), ("1", "4_bits or shared")):
+        _run(units, select)
+
+
+def _run(units, select):
     env = dict(os.environ, RI_TEST_KERNELS="emulated")
     env.pop("RI_KERNEL_LIBRARY", None)
+    env.pop("RI_EMU_COMPUTE_UNITS", None)
+    if units:
+        env["RI_EMU_COMPUTE_UNITS"] = units
     args = [sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider", os.path.join(HERE, "test_drafted_step_kernels_gpu.py")]
+    if select:
+        args += ["-k", select]
     try:
         import xdist  # noqa: F401
         args += ["-n", str(max(1, min(4, (os.cpu_count() or 2) // 2)))]

@@ -85,6 +85,8 @@ INT4 = [  # rows, n, k, group, zeros
     (1, 16, 128, 128, False), (1, 1, 8, 32, True), (3, 17, 136, 64, True), (8, 40, 1024, 128, True), (16, 33, 512, 32, True),
     (17, 48, 264, 32, False), (31, 20, 384, 256, True), (45, 50, 200, 64, False), (64, 64, 256, 128, True), (65, 18, 160, 32, True),
     (130, 16, 128, 64, True), (2, 100, 1408, 384, False), (5, 35, 2568, 128, True),
+    # (on a machine made small these go by the kernel that holds x: sixteen and more pieces of 128 columns, one tile and several a workgroup)
+    (16, 200, 2080, 64, True), (9, 331, 4096, 128, False), (1, 200, 1056, 32, True), (13, 900, 2048, 256, True), (16, 500, 3968, 32, False),
 ]
 
 
