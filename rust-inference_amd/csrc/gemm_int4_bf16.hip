@@ -35,8 +35,8 @@ union I4Frag {
 
 #define I4_PIECE 128             // columns a wavefront takes at a time: 16 bytes of codes a lane
 #define I4_ROWS 64               // rows of x a workgroup takes at most
-#define I4_NARROW 2              // tiles of 16 matrix rows a compute unit up to which a workgroup takes one of them
-#define I4_WIDE 12               // and up to which two (with up to 16 rows of x; then four)
+#define I4_NARROW 2              // tiles of 16 matrix rows a compute unit up to which eight wavefronts share a workgroup's tiles, not four
+#define I4_WIDE 12               // and up to which four wavefronts take two tiles, not four (with up to 16 rows of x)
 
 struct I4Args {
     void* out;
@@ -541,10 +541,14 @@ static void int4_by_group(const I4Args& a, int group, bool scale_f32, hipStream_
     else int4_launch<MT, NT, W, 4>(a, scale_f32, s);
 }
 
+// Few matrix rows leave a compute unit one or two workgroups: the length of K is split over eight wavefronts.  One row of x then takes a
+// tile a workgroup (4096 x 4096: 5.5 us, with two 7.1), more than 16 rows take two and read x half as often (45 x 5001 x 2568: 15.7 us,
+// with one 19 to 21; four wavefronts 17.4).  Many matrix rows fill the machine with four wavefronts (8 x 19456 x 2560: 20.7 us, with
+// eight 31), and very many with up to 16 rows of x read x a quarter as often by four tiles (16 x 151936 x 4096: 135 us, with two 165).
 template <int MT>
 static void int4_by_width(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
     const int tiles = (a.n + 15) / 16, units = ri_compute_units();
-    if (tiles <= I4_NARROW * units) int4_by_group<MT, 1, 8>(a, group, scale_f32, s);
+    if (tiles <= I4_NARROW * units) int4_by_group<MT, MT == 1 ? 1 : 2, 8>(a, group, scale_f32, s);
     else if (MT > 1 || tiles <= I4_WIDE * units) int4_by_group<MT, 2, 4>(a, group, scale_f32, s);
     else int4_by_group<MT, MT == 1 ? 4 : 2, 4>(a, group, scale_f32, s);
 }

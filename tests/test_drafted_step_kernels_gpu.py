@@ -88,6 +88,9 @@ INT4 = [  # rows, n, k, group, zeros
     # (on a machine made small these go by the kernel that holds x: sixteen and more pieces of 128 columns, one tile and several a workgroup)
     (16, 200, 2080, 64, True), (9, 331, 4096, 128, False), (1, 200, 1056, 32, True), (13, 900, 2048, 256, True), (16, 500, 3968, 32, False),
 ]
+if not EMULATED:                          # and on a whole one these do; the last by four tiles a workgroup and by two with four wavefronts
+    INT4 += [(3, 8300, 512, 128, True), (16, 9001, 1056, 64, False), (8, 16500, 2048, 32, True), (5, 8210, 4096, 256, True),
+             (16, 50001, 264, 32, True), (2, 8300, 4352, 128, False), (40, 8300, 200, 64, True), (20, 8200, 640, 128, False)]
 
 
 @pytest.mark.parametrize("rows, n, k, group, zeros", INT4)
@@ -200,17 +203,17 @@ class SharedCase:
         out, size, at = np.zeros((self.tokens, heads, dim)), np.zeros((self.tokens, heads, dim)), 0
         q = self.qkv[:, self.q_off:self.q_off + heads * dim].double().view(self.tokens, heads, dim).numpy()
         for b, (new, _) in enumerate(self.lens):
-            for i in range(new):
-                length = self.pos[at] + 1
-                pages = self.table[b, :-(-length // PAGE)].long()
-                for h in range(heads):
-                    keys = self.k[pages, h // per].reshape(-1, dim)[:length].double().numpy()
-                    values = self.v[pages, h // per].transpose(1, 2).reshape(-1, dim)[:length].double().numpy()
-                    s = keys @ q[at, h] * self.scale
-                    w = np.exp(s - s.max())
-                    w /= w.sum()
-                    out[at, h], size[at, h] = w @ values, w @ np.abs(values)
-                at += 1
+            pages = self.table[b, :-(-(max(self.pos[at:at + new], default=-1) + 1) // PAGE)].long()
+            for h in range(kv if new else 0):
+                keys = self.k[pages, h].reshape(-1, dim).double().numpy()
+                values = self.v[pages, h].transpose(1, 2).reshape(-1, dim).double().numpy()
+                for i in range(at, at + new):
+                    length, own = self.pos[i] + 1, slice(h * per, h * per + per)
+                    s = q[i, own] @ keys[:length].T * self.scale
+                    w = np.exp(s - s.max(1, keepdims=True))
+                    w /= w.sum(1, keepdims=True)
+                    out[i, own], size[i, own] = w @ values[:length], w @ np.abs(values[:length])
+            at += new
         return out.reshape(self.tokens, -1), size.reshape(self.tokens, -1)
 
     def check(self, got):
@@ -231,7 +234,12 @@ SHARED = [  # lens, shared, heads, kv, dim
     # (from 33 columns of a key head on the pages go through LDS, tiles of 64 and, from 65 on, 128; an odd last page, one pair, one page)
     ([(1, 2)] * 5, 288, 8, 1, 128), ([(2, 3)] * 5, 96, 8, 1, 128), ([(1, 1)] * 6, 32, 6, 1, 64), ([(3, 5)] * 15, 608, 3, 1, 32),
     ([(1, 4)] * 17, 544, 16, 2, 64), ([(2, 500), (0, 33), (1, 1)], 512, 8, 1, 128), ([(1, 2)] * 70, 64, 1, 1, 32), ([(40, 40), (9, 100)], 64, 4, 2, 64),
+    # no sequence, one without a new token, first and last
+    ([(0, 0), (2, 40), (0, 70)], 64, 4, 2, 64), ([(0, 5), (0, 0), (1, 3), (0, 0)], 224, 40, 1, 32),
 ]
+if not EMULATED:                          # runs of more than sixteen pages: from 129 columns on by eight wavefronts
+    SHARED += [([(3, 3)] * 6, 20480, 64, 8, 64), ([(2, 40), (1, 1)] * 6, 9600, 128, 8, 128), ([(20, 22)] * 7, 17472, 8, 8, 32),
+               ([(1, 50)] * 3, 33056, 16, 8, 128)]
 
 
 @pytest.mark.parametrize("lens, shared, heads, kv, dim", SHARED)
