@@ -34,9 +34,7 @@ union I4Frag {
 };
 
 #define I4_PIECE 128             // columns a wavefront takes at a time: 16 bytes of codes a lane
-#define I4_ROWS 64               // rows of x a workgroup takes at most
-#define I4_NARROW 2              // tiles of 16 matrix rows a compute unit up to which eight wavefronts share a workgroup's tiles, not four
-#define I4_WIDE 12               // and up to which four wavefronts take two tiles, not four (with up to 16 rows of x)
+#define I4_MANY 2                // tiles of 16 matrix rows a compute unit beyond which workgroups hold up to 16 rows of x
 
 struct I4Args {
     void* out;
@@ -137,9 +135,9 @@ template <int MT, int NT, int W, int STEPS, typename S>
 __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) {
     constexpr int USES = 4 / STEPS, ROUND = STEPS;            // groups that a piece meets; pieces that meet four groups
     constexpr int TURN = ROUND < 2 ? 2 : ROUND;               // pieces a turn of the loop: an even number, two buffers
-    constexpr bool X_TWICE = MT <= 2;
+    constexpr bool X_TWICE = MT == 1;
     const int lane = threadIdx.x & (RI_WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / RI_WAVE), i = lane & 15, j = lane >> 4;
-    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * I4_ROWS;
+    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
     const int full = a.k / I4_PIECE, pieces = (a.k + I4_PIECE - 1) / I4_PIECE;
     const size_t row_bytes = (size_t)a.k / 2;
     const S* scales = (const S*)a.scales;
@@ -527,30 +525,24 @@ static void int4_rows(const I4Args& a, int group, bool scale_f32, hipStream_t s)
 #undef I4_ROWS_LAUNCH
 }
 
-template <int MT, int NT, int W, int STEPS>
-static void int4_launch(const I4Args& a, bool scale_f32, hipStream_t s) {
-    const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.rows + I4_ROWS - 1) / I4_ROWS);
-    if (scale_f32) gemm_int4_kernel<MT, NT, W, STEPS, float><<<grid, W * RI_WAVE, 0, s>>>(a);
-    else gemm_int4_kernel<MT, NT, W, STEPS, bf16_t><<<grid, W * RI_WAVE, 0, s>>>(a);
-}
-
 template <int MT, int NT, int W>
-static void int4_by_group(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
-    if (group == 32) int4_launch<MT, NT, W, 1>(a, scale_f32, s);
-    else if (group == 64) int4_launch<MT, NT, W, 2>(a, scale_f32, s);
-    else int4_launch<MT, NT, W, 4>(a, scale_f32, s);
+static void int4_tiles(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
+    const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.rows + 16 * MT - 1) / (16 * MT));
+#define I4_LAUNCH(STEPS)                                                                                         \
+    do {                                                                                                         \
+        if (scale_f32) gemm_int4_kernel<MT, NT, W, STEPS, float><<<grid, W * RI_WAVE, 0, s>>>(a);                \
+        else gemm_int4_kernel<MT, NT, W, STEPS, bf16_t><<<grid, W * RI_WAVE, 0, s>>>(a);                         \
+    } while (0)
+    if (group == 32) I4_LAUNCH(1);
+    else if (group == 64) I4_LAUNCH(2);
+    else I4_LAUNCH(4);
+#undef I4_LAUNCH
 }
 
-// Few matrix rows leave a compute unit one or two workgroups: the length of K is split over eight wavefronts.  One row of x then takes a
-// tile a workgroup (4096 x 4096: 5.5 us, with two 7.1), more than 16 rows take two and read x half as often (45 x 5001 x 2568: 15.7 us,
-// with one 19 to 21; four wavefronts 17.4).  Many matrix rows fill the machine with four wavefronts (8 x 19456 x 2560: 20.7 us, with
-// eight 31), and very many with up to 16 rows of x read x a quarter as often by four tiles (16 x 151936 x 4096: 135 us, with two 165).
-template <int MT>
-static void int4_by_width(const I4Args& a, int group, bool scale_f32, hipStream_t s) {
-    const int tiles = (a.n + 15) / 16, units = ri_compute_units();
-    if (tiles <= I4_NARROW * units) int4_by_group<MT, MT == 1 ? 1 : 2, 8>(a, group, scale_f32, s);
-    else if (MT > 1 || tiles <= I4_WIDE * units) int4_by_group<MT, 2, 4>(a, group, scale_f32, s);
-    else int4_by_group<MT, MT == 1 ? 4 : 2, 4>(a, group, scale_f32, s);
+// What a compute unit does: the rounds in which the workgroups of `tall` x `wide` tiles go, times their tiles.
+static long int4_rounds(const I4Args& a, int tall, int wide) {
+    const long rows = (a.rows + 16 * tall - 1) / (16 * tall), cols = (a.n + 16 * wide - 1) / (16 * wide), units = ri_compute_units();
+    return (rows * cols + units - 1) / units * tall * wide;
 }
 
 extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const void* codes, const void* scales, int scale_dtype,
@@ -559,7 +551,7 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
     RI_REQUIRE(k % 8 == 0, "gemm_int4: k %d is no multiple of 8", k);
     RI_REQUIRE(group == 32 || group == 64 || (group > 0 && group % 128 == 0),
                "gemm_int4: groups of %d columns, 32, 64 and multiples of 128 are taken", group);
-    RI_REQUIRE(rows <= 65535 * I4_ROWS && n <= 0x7fffffff - 64, "gemm_int4: %d rows, n %d are too many", rows, n);
+    RI_REQUIRE(rows <= 65535 * 16 && n <= 0x7fffffff - 64, "gemm_int4: %d rows, n %d are too many", rows, n);
     RI_REQUIRE((out_dtype == RI_F32 || out_dtype == RI_BF16) && (scale_dtype == RI_F32 || scale_dtype == RI_BF16), "gemm_int4: unknown dtype");
     RI_REQUIRE(out && x && codes && scales, "gemm_int4: an operand is missing");
     RI_REQUIRE((uintptr_t)x % 16 == 0, "gemm_int4: x must start on a 16-byte boundary");
@@ -569,13 +561,24 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
                       group >= 128 ? group / 128 : 1, out_dtype == RI_F32};
     const bool f = scale_dtype == RI_F32;
     const hipStream_t s = (hipStream_t)stream;
-    const int pieces = (k + I4_PIECE - 1) / I4_PIECE;
-    if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && (n + 15) / 16 > I4_NARROW * ri_compute_units()) {
+    const int pieces = (k + I4_PIECE - 1) / I4_PIECE, tiles = (n + 15) / 16, units = ri_compute_units();
+    // (8 x 19456 x 2560: 12.6 us; by tiles 20.7.  16 x 151936 x 4096: 77 us; by tiles 135.)
+    if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && tiles > I4_MANY * units) {
         if (pieces <= 16) int4_rows<2, 2>(a, group, f, s);
         else int4_rows<4, 1>(a, group, f, s);
-    } else if (rows <= 16) int4_by_width<1>(a, group, f, s);
-    else if (rows <= 32) int4_by_width<2>(a, group, f, s);
-    else int4_by_width<4>(a, group, f, s);
+    } else if ((long)tiles * ((rows + 15) / 16) <= units) {
+        // A tile a workgroup, and eight wavefronts on the length of K, where every one has a compute unit to itself: 4096 x 4096 takes
+        // 5.6 us with one row and 8.5 with 16 (two tiles by four wavefronts: 8.2 and 9.8; four tiles: 11.7 and 13.3).
+        int4_tiles<1, 1, 8>(a, group, f, s);
+    } else {
+        // Else the tiles that leave the compute units the least to do, and up to an eighth more of it where they are larger: x, or the
+        // codes, are then read less often.  In us, 1 x 2, 1 x 4 and 4 x 2 tiles: 45 x 2560 x 9728 17.7, 24.4, 36.8; 48 x 19456 x 2560
+        // 33.0, 27.8, 33.4; 64 x 151936 x 2560 284, 225, 214; 256 x 4096 x 4096 57, 45, 40.  (Eight wavefronts: up to 8% more.)
+        const long two = int4_rounds(a, 1, 2), four = int4_rounds(a, 1, 4), eight = int4_rounds(a, 4, 2);
+        if (8 * eight <= 9 * min(two, four)) int4_tiles<4, 2, 4>(a, group, f, s);
+        else if (8 * four <= 9 * two) int4_tiles<1, 4, 4>(a, group, f, s);
+        else int4_tiles<1, 2, 4>(a, group, f, s);
+    }
     RI_LAUNCH_CHECK("gemm_int4");
     return 0;
 }

@@ -88,9 +88,10 @@ INT4 = [  # rows, n, k, group, zeros
     # (on a machine made small these go by the kernel that holds x: sixteen and more pieces of 128 columns, one tile and several a workgroup)
     (16, 200, 2080, 64, True), (9, 331, 4096, 128, False), (1, 200, 1056, 32, True), (13, 900, 2048, 256, True), (16, 500, 3968, 32, False),
 ]
-if not EMULATED:                          # and on a whole one these do; the last by four tiles a workgroup and by two with four wavefronts
+if not EMULATED:                          # and on a whole one these do; the last by two, four and four times two tiles
     INT4 += [(3, 8300, 512, 128, True), (16, 9001, 1056, 64, False), (8, 16500, 2048, 32, True), (5, 8210, 4096, 256, True),
-             (16, 50001, 264, 32, True), (2, 8300, 4352, 128, False), (40, 8300, 200, 64, True), (20, 8200, 640, 128, False)]
+             (16, 50001, 264, 32, True), (2, 8300, 4352, 128, False), (40, 8300, 200, 64, True), (20, 8200, 640, 128, False),
+             (45, 2560, 1032, 32, True), (49, 33001, 136, 64, True), (256, 4100, 512, 128, False), (129, 5000, 264, 32, True)]
 
 
 @pytest.mark.parametrize("rows, n, k, group, zeros", INT4)
