@@ -13,6 +13,8 @@
 //
 // Keys and values behind a sequence's last token are whatever the page held before: they are taken as zeros, so that an
 // infinity or NaN there reaches nothing.
+#include <float.h>
+
 #include "attention_mfma.h"
 
 #define SH_OWN_PAGES 16          // pages of a chunk of a sequence's own keys: this many, or half where that leaves compute units empty
@@ -496,7 +498,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE(max_len >= 1 && max_len <= (long)table_width * PAGE, "attention_shared: sequences of up to %d tokens, tables of %d pages", max_len, table_width);
     RI_REQUIRE(kv_heads <= 65535 && tokens <= 65535 && heads <= 65535, "attention_shared: %d tokens, %d heads exceed one launch", tokens, heads);
     RI_REQUIRE((long)table_width * PAGE < 0x7fffffff, "attention_shared: page table width %d", table_width);
-    RI_REQUIRE(scale > 0.f, "attention_shared: scale %g is not positive", (double)scale);
+    RI_REQUIRE(scale > 0.f && scale <= FLT_MAX, "attention_shared: scale %g is no positive number", (double)scale);
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
     const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
     const long of_shared = (long)p.splits * p.tiles * kv_heads, of_own = (long)p.own_chunks * p.own_tiles * seqs * kv_heads;

@@ -71,7 +71,7 @@ __device__ __forceinline__ double exp2_nonpositive(double t) {
 // The exponentials of a row's (or a chunk's) entries over that of its largest one.  Ordinary temperatures: with M the whole
 // number next to m s, 2^(x s - M) takes thirteen float64 instructions, since x s + (1.5 * 2^52 - M) has the whole part in
 // place at once, and x is held in float32 to what the exponent has room for: lo, where the result is 2^-1000 up to the
-// rounding of lo.  That wants |M| below 2^27; `plain` does without.  NaN and what lies at lo or below is a masked entry, an
+// rounding of lo.  That wants |M| below 2^27 and lo in float32's range; `plain` does without.  NaN and what lies at lo or below is a masked entry, an
 // infinite logit the largest finite number.
 struct Scale { double s, inv; };                 // log2(e) / T and its inverse
 struct Exps {
@@ -84,9 +84,10 @@ __device__ __forceinline__ Exps exps_below(double m, Scale by) {
     const double whole = rint(m * by.s);
     r.s = by.s;
     r.top = (float)m;
-    r.plain = !(fabs(whole) < 134217728.0);
+    const double lo = (whole - 1000.0) * by.inv;
+    r.plain = !(fabs(whole) < 134217728.0 && lo >= -FLT_MAX);
     r.c = VER_MAGIC - whole;
-    r.lo = (float)((whole - 1000.0) * by.inv);
+    r.lo = (float)lo;
     r.back = r.plain ? 1.0 : exp2_parts(fma(-m, by.s, whole), 0.0);
     return r;
 }
@@ -557,7 +558,7 @@ extern "C" int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* lo
     RI_REQUIRE(ri_verify_drafts_workspace_words(seqs, rows, vocab, draft_logits != nullptr) > 0,
                "verify_drafts: %d rows of a vocabulary of %d are too much for one call", rows, vocab);
     RI_REQUIRE(accepted && out && logits && tokens && cu_seqlens && workspace, "verify_drafts: an operand is missing");
-    RI_REQUIRE(temperature == temperature, "verify_drafts: the temperature is no number");
+    RI_REQUIRE(temperature < INFINITY, "verify_drafts: the temperature is no finite number");      // (nor is NaN)
     const hipStream_t s = (hipStream_t)stream;
     const int chunks = verify_chunks(vocab);
     const bool wide = vocab % 4 == 0 && (uintptr_t)logits % 16 == 0 && (uintptr_t)draft_logits % 16 == 0;

@@ -294,7 +294,7 @@ def test_attention_over_shared_pages_refuses_what_it_does_not_take(ops):
                    dict(qkv=guarded(c.qkv.float())), dict(k=guarded(c.k[:, :1])), dict(qkv=guarded(c.qkv[:, :200]))):
         with pytest.raises(InferenceError):
             c.run(ops, **change)
-    for name, value in (("dim", 48), ("heads", 5), ("q_off", 4), ("scale", 0.0), ("max_new", 0)):
+    for name, value in (("dim", 48), ("heads", 5), ("q_off", 4), ("scale", 0.0), ("scale", float("inf")), ("max_new", 0)):
         kept = getattr(c, name)
         setattr(c, name, value)
         with pytest.raises(InferenceError):
@@ -426,6 +426,22 @@ def test_temperatures_at_the_ends_of_their_range(ops, temperature, with_draft):
     same(verify(ops, logits, draft, tokens, counts, u, temperature), want)
 
 
+@pytest.mark.parametrize("temperature", [1e33, 1e35, 3e36, 1e38, 1e300])
+@pytest.mark.parametrize("large", [False, True])
+def test_very_high_temperatures_with_masked_entries(ops, temperature, large):
+    """Logits as large as the temperature, up to float32's ends, or ordinary ones beside it; what is masked weighs nothing still."""
+    counts, vocab = [3, 2, 5], 4500
+    rng = np.random.default_rng(13)
+    logits, draft, tokens, u = drafted(counts, vocab, 1.0, True, 13)
+    if large:
+        logits, draft = (np.clip(0.5 * a.astype(np.float64) * min(temperature, 1e38), -3.4e38, 3.4e38).astype(np.float32) for a in (logits, draft))
+    for a in (logits, draft):
+        a[rng.random(a.shape) < 0.4] = -np.inf
+        a[rng.random(a.shape) < 0.1] = np.nan
+    for d in (draft, None):
+        same(verify(ops, logits, d, tokens, counts, u, temperature), plain_verify(logits, d, tokens, counts, u, temperature, margin=1e-9))
+
+
 @pytest.mark.parametrize("vocab", [411, 5000])
 def test_drafts_of_the_target_itself_all_stand(ops, vocab):
     counts = [6, 1, 9]
@@ -517,7 +533,7 @@ def test_drafts_are_refused_where_an_operand_does_not_fit(ops):
     good = dict(logits=t(logits), tokens=i32(tokens), cu=i32([0, 3, 5]), u=t(u), temperature=1.0, draft=t(draft))
     for change in (dict(u=None), dict(u=t(u[:4])), dict(tokens=i32(tokens[:4])), dict(tokens=guarded(torch.tensor(tokens))), dict(draft=t(draft[:4])),
                    dict(draft=t(draft[:, :39])), dict(logits=t(logits).double()), dict(logits=t(logits)[0]), dict(cu=i32([0])),
-                   dict(logits=t(logits)[:0]), dict(temperature=float("nan")), dict(logits=t(np.concatenate([logits, logits], 1))[:, :40])):
+                   dict(logits=t(logits)[:0]), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(logits=t(np.concatenate([logits, logits], 1))[:, :40])):
         a = dict(good, **change)
         with pytest.raises(InferenceError):
             ops.verify_drafts(a["logits"], a["tokens"], a["cu"], a["u"], a["temperature"], a["draft"])
