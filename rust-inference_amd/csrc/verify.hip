@@ -16,9 +16,9 @@
 //
 // Four launches.  `stats` cuts every row that is asked about into chunks of 4,096 entries, a wavefront each, and leaves a
 // chunk's largest logit and its sum of exponentials: the one pass over the logits.  `end` (a workgroup a sequence) joins the
-// rows' chunks, a row a wavefront, until a draft falls.  `weigh` sums what the entries of every chunk weigh in the draw
-// of the last token, `pick` (a workgroup a sequence) finds the chunk and in it the token.  Greedy steps need two: the
-// chunks' best entries, then the walk.
+// rows' chunks, a row a wavefront, until a draft falls; where there is little to do `weigh` does that beside its own work.
+// `weigh` sums what the entries of every chunk weigh in the draw of the last token, `pick` (a workgroup a sequence) finds the
+// chunk and in it the token.  Greedy steps need two: the chunks' best entries, then the walk.
 // Every sum has one order, so the same inputs give the same tokens.
 #include <float.h>
 
@@ -262,16 +262,12 @@ __device__ __forceinline__ Weights weigh_entry(const Weigher& w, float x, float 
     return {id == w.less ? 0.0 : p, p};
 }
 
-__global__ __launch_bounds__(VER_THREADS) void verify_end(Ending* __restrict__ endings, const ChunkStats* __restrict__ stats,
-                                                          const float* __restrict__ logits, const float* __restrict__ draft,
-                                                          const int32_t* __restrict__ tokens, const int32_t* __restrict__ cu,
-                                                          const float* __restrict__ uniform, int rows, int vocab, int chunks, Scale scale) {
-    const int b = blockIdx.x, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
+// Where a sequence's walk ends, by a workgroup: four rows at a time, a wavefront each, until one ends it; the last row always does.
+__device__ __forceinline__ Ending ending_of(const ChunkStats* __restrict__ stats, const float* __restrict__ logits,
+                                            const float* __restrict__ draft, const int32_t* __restrict__ tokens,
+                                            const float* __restrict__ uniform, int r0, int r1, int rows, int vocab, int chunks, Scale scale) {
+    const int lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
     __shared__ Ending tried[VER_WAVES];
-    int r0, r1;
-    rows_of(cu, b, rows, r0, r1);
-    if (r0 == r1) return;
-    // four rows at a time, a wavefront each, until one ends the walk; the last row always does
     for (int base = r0;; base += VER_WAVES) {
         const int row = base + wave;
         Ending mine = {{0.0, 0.0}, {0.0, 0.0}, -1, -1, 0, 0};
@@ -300,10 +296,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_end(Ending* __restrict__ e
         int first = -1;
         for (int w = VER_WAVES - 1; w >= 0; --w)
             if (tried[w].row >= 0) first = w;
-        if (first >= 0) {
-            if (threadIdx.x == 0) endings[b] = tried[first];
-            return;
-        }
+        if (first >= 0) return tried[first];
         __syncthreads();
     }
 }
@@ -320,17 +313,32 @@ __device__ __forceinline__ Weights sum_weights(const Weigher& by, const float (&
     return sum;
 }
 
-template <bool WIDE>
-__global__ __launch_bounds__(VER_THREADS) void verify_weigh(Weights* __restrict__ masses, const Ending* __restrict__ endings,
-                                                            const float* __restrict__ logits, const float* __restrict__ draft,
-                                                            const int32_t* __restrict__ cu, int rows, int vocab, int chunks, Scale scale) {
+__global__ __launch_bounds__(VER_THREADS) void verify_end(Ending* __restrict__ endings, const ChunkStats* __restrict__ stats,
+                                                          const float* __restrict__ logits, const float* __restrict__ draft,
+                                                          const int32_t* __restrict__ tokens, const int32_t* __restrict__ cu,
+                                                          const float* __restrict__ uniform, int rows, int vocab, int chunks, Scale scale) {
+    int r0, r1;
+    rows_of(cu, blockIdx.x, rows, r0, r1);
+    if (r0 == r1) return;
+    const Ending end = ending_of(stats, logits, draft, tokens, uniform, r0, r1, rows, vocab, chunks, scale);
+    if (threadIdx.x == 0) endings[blockIdx.x] = end;
+}
+
+// ENDS: every workgroup finds its sequence's ending for itself, the first chunk's leaves it for `pick`.
+template <bool WIDE, bool ENDS>
+__global__ __launch_bounds__(VER_THREADS) void verify_weigh(Weights* __restrict__ masses, Ending* __restrict__ endings,
+                                                            const ChunkStats* __restrict__ stats, const float* __restrict__ logits,
+                                                            const float* __restrict__ draft, const int32_t* __restrict__ tokens,
+                                                            const int32_t* __restrict__ cu, const float* __restrict__ uniform, int rows,
+                                                            int vocab, int chunks, Scale scale) {
     constexpr int EACH = VER_CHUNK / VER_THREADS;
     const int chunk = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & (RI_WAVE - 1), wave = threadIdx.x / RI_WAVE;
     __shared__ Weights sums[VER_WAVES];
     int r0, r1;
     rows_of(cu, b, rows, r0, r1);
     if (r0 == r1) return;
-    const Ending end = endings[b];
+    const Ending end = ENDS ? ending_of(stats, logits, draft, tokens, uniform, r0, r1, rows, vocab, chunks, scale) : endings[b];
+    if (ENDS && chunk == 0 && threadIdx.x == 0) endings[b] = end;
     const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
     const Weigher by = weigher(end, draft != nullptr, scale);
     float x[EACH], qx[EACH];
@@ -384,8 +392,10 @@ __device__ __forceinline__ double wave_upto(double v) {
 struct Drawn { double target, before; int chunk, whole; };
 __device__ __forceinline__ Drawn draw_chunk(const Weights* __restrict__ mine, int chunks, double u) {
     const int lane = threadIdx.x & (RI_WAVE - 1);
-    double left = 0.0, whole = 0.0;                           // of all chunks
-    for (int c0 = 0; c0 < chunks; c0 += RI_WAVE) {
+    const Weights first = lane < chunks ? mine[lane] : Weights{0.0, 0.0};
+    const Weights first_upto = {wave_upto(first.left), wave_upto(first.whole)};
+    double left = __shfl(first_upto.left, RI_WAVE - 1, RI_WAVE), whole = __shfl(first_upto.whole, RI_WAVE - 1, RI_WAVE);       // of all chunks
+    for (int c0 = RI_WAVE; c0 < chunks; c0 += RI_WAVE) {
         const Weights w = c0 + lane < chunks ? mine[c0 + lane] : Weights{0.0, 0.0};
         left += __shfl(wave_upto(w.left), RI_WAVE - 1, RI_WAVE);
         whole += __shfl(wave_upto(w.whole), RI_WAVE - 1, RI_WAVE);
@@ -397,8 +407,12 @@ __device__ __forceinline__ Drawn draw_chunk(const Weights* __restrict__ mine, in
     d.chunk = 0;
     double carried = 0.0;
     for (int c0 = 0; c0 < chunks; c0 += RI_WAVE) {
-        const Weights w = c0 + lane < chunks ? mine[c0 + lane] : Weights{0.0, 0.0};
-        const double own = d.whole ? w.whole : w.left, upto = carried + wave_upto(own);
+        double own = d.whole ? first.whole : first.left, upto = d.whole ? first_upto.whole : first_upto.left;
+        if (c0 > 0) {
+            const Weights w = c0 + lane < chunks ? mine[c0 + lane] : Weights{0.0, 0.0};
+            own = d.whole ? w.whole : w.left;
+            upto = carried + wave_upto(own);
+        }
         const unsigned long long some = __ballot(own > 0.0), past = __ballot(own > 0.0 && upto > d.target);
         const unsigned long long take = past ? past & (0ull - past) : some;       // the first past the target, else the last of some
         if (take) {
@@ -580,9 +594,19 @@ extern "C" int ri_verify_drafts(int32_t* accepted, int32_t* out, const float* lo
     const dim3 grid(chunks, rows, draft_logits ? 2 : 1), grid2(chunks, seqs);
     if (wide) verify_stats<true><<<grid, RI_WAVE, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
     else verify_stats<false><<<grid, RI_WAVE, 0, s>>>(stats, logits, draft_logits, cu_seqlens, seqs, rows, vocab, chunks, scale);
-    verify_end<<<seqs, VER_THREADS, 0, s>>>(endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, rows, vocab, chunks, scale);
-    if (wide) verify_weigh<true><<<grid2, VER_THREADS, 0, s>>>(masses, endings, logits, draft_logits, cu_seqlens, rows, vocab, chunks, scale);
-    else verify_weigh<false><<<grid2, VER_THREADS, 0, s>>>(masses, endings, logits, draft_logits, cu_seqlens, rows, vocab, chunks, scale);
+#define VERIFY_WEIGH(WIDE, ENDS)                                                                                              \
+    verify_weigh<WIDE, ENDS><<<grid2, VER_THREADS, 0, s>>>(masses, endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, \
+                                                           rows, vocab, chunks, scale)
+    // Few chunks: a launch less (one sequence of 5 rows x 151,936: 23 us, with `end` 26; 64 of them: 113 and 109).
+    if ((long)chunks * seqs <= 2L * ri_compute_units()) {
+        if (wide) VERIFY_WEIGH(true, true);
+        else VERIFY_WEIGH(false, true);
+    } else {
+        verify_end<<<seqs, VER_THREADS, 0, s>>>(endings, stats, logits, draft_logits, tokens, cu_seqlens, uniform, rows, vocab, chunks, scale);
+        if (wide) VERIFY_WEIGH(true, false);
+        else VERIFY_WEIGH(false, false);
+    }
+#undef VERIFY_WEIGH
     verify_pick<<<seqs, VER_PICK_THREADS, 0, s>>>(accepted, out, masses, endings, logits, draft_logits, tokens, cu_seqlens, uniform, seqs,
                                                   rows, vocab, chunks, scale);
     RI_LAUNCH_CHECK("verify_drafts");
