@@ -34,7 +34,6 @@ union I4Frag {
 };
 
 #define I4_PIECE 128             // columns a wavefront takes at a time: 16 bytes of codes a lane
-#define I4_MANY 2                // tiles of 16 matrix rows a compute unit beyond which workgroups hold up to 16 rows of x
 
 struct I4Args {
     void* out;
@@ -562,8 +561,9 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
     const bool f = scale_dtype == RI_F32;
     const hipStream_t s = (hipStream_t)stream;
     const int pieces = (k + I4_PIECE - 1) / I4_PIECE, tiles = (n + 15) / 16, units = ri_compute_units();
-    // (8 x 19456 x 2560: 12.6 us; by tiles 20.7.  16 x 151936 x 4096: 77 us; by tiles 135.)
-    if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && tiles > I4_MANY * units) {
+    // More tiles of matrix rows than compute units: x is held and the matrix walked.  In us, so and by tiles: 1 x 8192 x 4096 7.1 and 8.5,
+    // 4 x 12288 x 4096 8.8 and 13.4, 16 x 24576 x 4096 15.5 and 25, 16 x 151936 x 4096 77 and 135; 4 x 5120 x 2560 level.
+    if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && tiles > units) {
         if (pieces <= 16) int4_rows<2, 2>(a, group, f, s);
         else int4_rows<4, 1>(a, group, f, s);
     } else if ((long)tiles * ((rows + 15) / 16) <= units) {
