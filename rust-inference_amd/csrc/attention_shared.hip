@@ -82,20 +82,25 @@ __device__ __forceinline__ int first_ids(const int32_t* table, int page0, int pa
     return table[min(page0 + (int)(threadIdx.x >> 6) + (int)(threadIdx.x & 63) * W, pages - 1)];
 }
 
-// Few columns: a tile of 16 over the pages page0 .. page1, which the wavefronts take in turn; they meet in LDS.
-template <int DH, int W, int SLOTS>
+// Few columns: a tile of 16 NT over the pages page0 .. page1, which the wavefronts take in turn; they meet in LDS.
+template <int DH, int NT, int W, int SLOTS>
 __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, const int32_t* table, int kvh, int slot,
                                             int first_token, int col0, int cols, int page0, int page1, int last_key, int ids) {
     constexpr int LD = SharedLds<DH, W, SLOTS>::LD;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
-    Columns<DH, 1> c;
-    init_columns<DH, 1>(c);
-    const int col = col0 + i;
-    const Place place = place_of(a, first_token, kvh, min(col, cols - 1));
-    c.qpos[0] = min(a.tok_pos[place.token], last_key);
-    const bf16_t* q = a.q + (size_t)place.token * a.q_stride + place.head * DH + jg * 8;
+    Columns<DH, NT> c;
+    init_columns<DH, NT>(c);
+    Place place[NT];
+    int min_qpos = last_key;
 #pragma unroll
-    for (int ks = 0; ks < DH / 32; ++ks) c.q[0][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
+    for (int n = 0; n < NT; ++n) {
+        place[n] = place_of(a, first_token, kvh, min(col0 + 16 * n + i, cols - 1));
+        c.qpos[n] = min(a.tok_pos[place[n].token], last_key);
+        min_qpos = min(min_qpos, c.qpos[n]);
+        const bf16_t* q = a.q + (size_t)place[n].token * a.q_stride + place[n].head * DH + jg * 8;
+#pragma unroll
+        for (int ks = 0; ks < DH / 32; ++ks) c.q[n][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
+    }
     // The next page's keys are asked for when this one's are used up, its values likewise: a page is on its way all the time.
     // (Behind the last page: a line of it.)
     Frag kf[2][DH / 32], vf[DH / 16];
@@ -138,46 +143,50 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W
         for (; page < page1; page += W) {
             const int last = last_key - page * PAGE;
             const bool more = page + W < page1;
-            Frag p[1];
+            Frag p[NT];
             if (last < PAGE - 1) drop_keys<DH>(kf, last, lane);
-            scores_and_weights<DH, 1>(c, kf, p, page, lane, a.scale_log2, !__any(c.qpos[0] < page * PAGE + PAGE - 1));
+            scores_and_weights<DH, NT>(c, kf, p, page, lane, a.scale_log2, !__any(min_qpos < page * PAGE + PAGE - 1));
             const long next = phys_of(page + W);
             load_keys(next, more);
             if (last < PAGE - 1) drop_values<DH>(vf, last, lane);
-            weighted_values<DH, 1>(c, vf, p);
+            weighted_values<DH, NT>(c, vf, p);
             load_values(next, more);
         }
     }
-    finish_columns<DH, 1>(c);
+    finish_columns<DH, NT>(c);
     auto& meet = lds.meet;
-    if (jg == 0) {
-        meet.m[wave][i] = c.m[0];
-        meet.l[wave][i] = c.l[0];
-    }
-    __syncthreads();
-    float m = meet.m[0][i], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < W; ++w) m = fmaxf(m, meet.m[w][i]);
-    const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int w = 0; w < W; ++w) l += __builtin_amdgcn_exp2f(meet.m[w][i] - ref) * meet.l[w][i];
-    const float mine = __builtin_amdgcn_exp2f(c.m[0] - ref);
-#pragma unroll
-    for (int dt = 0; dt < DH / 16; ++dt)
-        *reinterpret_cast<float4*>(&meet.o[wave][i * LD + dt * 16 + jg * 4]) =
-            make_float4(c.o[0][dt][0] * mine, c.o[0][dt][1] * mine, c.o[0][dt][2] * mine, c.o[0][dt][3] * mine);
-    if (wave == 0 && jg == 0 && col < cols) a.stats[result_at(a, slot, place)] = make_float2(m, l);
-    __syncthreads();
-    for (int at = threadIdx.x; at < 16 * DH / 4; at += W * 64) {
-        const int r = at / (DH / 4), d = at % (DH / 4) * 4;
-        if (col0 + r >= cols) break;
-        float4 o = *reinterpret_cast<const float4*>(&meet.o[0][r * LD + d]);
-#pragma unroll
-        for (int w = 1; w < W; ++w) {
-            const float4 more = *reinterpret_cast<const float4*>(&meet.o[w][r * LD + d]);
-            o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
+    for (int n = 0; n < NT; ++n) {
+        if (jg == 0) {
+            meet.m[wave][i] = c.m[n];
+            meet.l[wave][i] = c.l[n];
         }
-        *reinterpret_cast<float4*>(a.sums + result_at(a, slot, place_of(a, first_token, kvh, col0 + r)) * DH + d) = o;
+        __syncthreads();
+        float m = meet.m[0][i], l = 0.f;
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = fmaxf(m, meet.m[w][i]);
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int w = 0; w < W; ++w) l += __builtin_amdgcn_exp2f(meet.m[w][i] - ref) * meet.l[w][i];
+        const float mine = __builtin_amdgcn_exp2f(c.m[n] - ref);
+#pragma unroll
+        for (int dt = 0; dt < DH / 16; ++dt)
+            *reinterpret_cast<float4*>(&meet.o[wave][i * LD + dt * 16 + jg * 4]) =
+                make_float4(c.o[n][dt][0] * mine, c.o[n][dt][1] * mine, c.o[n][dt][2] * mine, c.o[n][dt][3] * mine);
+        if (wave == 0 && jg == 0 && col0 + 16 * n + i < cols) a.stats[result_at(a, slot, place[n])] = make_float2(m, l);
+        __syncthreads();
+        for (int at = threadIdx.x; at < 16 * DH / 4; at += W * 64) {
+            const int r = at / (DH / 4), d = at % (DH / 4) * 4, col = col0 + 16 * n + r;
+            if (col >= cols) break;
+            float4 o = *reinterpret_cast<const float4*>(&meet.o[0][r * LD + d]);
+#pragma unroll
+            for (int w = 1; w < W; ++w) {
+                const float4 more = *reinterpret_cast<const float4*>(&meet.o[w][r * LD + d]);
+                o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
+            }
+            *reinterpret_cast<float4*>(a.sums + result_at(a, slot, place_of(a, first_token, kvh, col)) * DH + d) = o;
+        }
+        if (n + 1 < NT) __syncthreads();                      // (the next sixteen meet in the same place)
     }
 }
 
@@ -346,7 +355,7 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
 }
 
 // A sequence's own chunk, by its number among all (key heads fastest, then tiles, chunks, sequences).
-template <int DH, int W>
+template <int DH, int NT, int W>
 __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 0>& lds, int item) {
     const int kvh = item % a.kv_heads;
     item /= a.kv_heads;
@@ -358,28 +367,28 @@ __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 
     const int ids = first_ids<W>(table, page0, a.table_width);
     const int first = min(max(a.cu_seqlens[seq], 0), a.tokens), behind = min(max(a.cu_seqlens[seq + 1], first), a.tokens);
     const int cols = (behind - first) * (a.heads / a.kv_heads);
-    if (tile * 16 >= cols) return;
+    if (tile * 16 * NT >= cols) return;
     const int last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
     const int page1 = min(page0 + a.own_pages, last_key / PAGE + 1);
     if (page0 >= page1) return;
-    few_columns<DH>(a, lds, table, kvh, a.splits + chunk, first, tile * 16, cols, page0, page1, last_key, ids);
+    few_columns<DH, NT>(a, lds, table, kvh, a.splits + chunk, first, tile * 16 * NT, cols, page0, page1, last_key, ids);
 }
 
 // Few columns in all: the runs of the shared pages and the sequences' own chunks, a workgroup each; with more (ALL false) the own
 // chunks alone.
-template <int DH, bool ALL, int W>
-__global__ void __launch_bounds__(W * 64, 3) attn_shared_few_kernel(const SharedArgs a) {
+template <int DH, bool ALL, int NT, int W>
+__global__ void __launch_bounds__(W * 64, NT == 1 ? 3 : 2) attn_shared_few_kernel(const SharedArgs a) {
     __shared__ __attribute__((aligned(16))) SharedLds<DH, W, 0> lds;
     const int of_tile = a.splits * a.kv_heads, shared_items = ALL ? of_tile * a.tiles : 0;
     int item = blockIdx.x;
     if (item >= shared_items) {
-        own_chunk<DH>(a, lds, item - shared_items);
+        own_chunk<DH, NT>(a, lds, item - shared_items);
         return;
     }
     const int tile = item / of_tile;
     item -= tile * of_tile;
     const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads, page0 = slot * a.pages_per_split;
-    few_columns<DH>(a, lds, a.page_table, kvh, slot, 0, tile * 16, a.tokens * (a.heads / a.kv_heads), page0,
+    few_columns<DH, NT>(a, lds, a.page_table, kvh, slot, 0, tile * 16 * NT, a.tokens * (a.heads / a.kv_heads), page0,
                     min(page0 + a.pages_per_split, a.shared_pages), a.shared_pages * PAGE - 1,
                     first_ids<W>(a.page_table, page0, a.shared_pages));
 }
@@ -448,8 +457,10 @@ __global__ void __launch_bounds__(SH_JOIN) attn_shared_join_kernel(bf16_t* __res
     *to = uint2{pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv)};
 }
 
-struct SharedPlan { int nt, waves, splits, pages_per_split, tiles, own_tiles, own_chunks, own_pages; };
+struct SharedPlan { int nt, few, waves, splits, pages_per_split, tiles, own_tiles, own_chunks, own_pages; };
 
+// A sequence that brings more than 16 columns takes them 32 a workgroup, with fewer wavefronts a compute unit, so that its own keys are read
+// half as often: 16 sequences of up to 5 tokens of 4 heads a key head, 20 to 900 own keys, 14.0 us (tiles of 16: 15.7).
 // More than 32 columns a key head take the form of many columns: workgroups of four wavefronts with a tile of 64 or, from 65 columns on,
 // 128, two of them a compute unit; from 129 columns on, where a run is longer than SH_SHORT_PAGES, of eight with 256, whose copies
 // have three turns to arrive instead of one.  us with four : eight wavefronts: 32 sequences of 64 heads behind 131,072 tokens (runs of 128
@@ -461,12 +472,13 @@ static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_page
     const int group = heads / kv_heads;
     const long cols = (long)tokens * group;
     p.nt = cols <= 32 ? 0 : cols <= 64 ? 1 : 2;
-    p.own_tiles = (int)(((long)max_new * group + 15) / 16);
+    p.few = (long)max_new * group <= 16 ? 1 : 2;
+    p.own_tiles = (int)(((long)max_new * group + 16 * p.few - 1) / (16 * p.few));
     const int own = max_len - shared_pages * PAGE;
     p.own_pages = (long)seqs * kv_heads * p.own_tiles <= ri_compute_units() ? SH_OWN_PAGES / 2 : SH_OWN_PAGES;      // (max_len changes no sum)
     p.own_chunks = own > 0 ? (own + p.own_pages * PAGE - 1) / (p.own_pages * PAGE) : 0;
     for (p.waves = cols <= 128 ? 4 : 8;; p.waves = 4) {
-        const int of_wg = p.nt == 0 ? 16 : 16 * p.waves * p.nt;
+        const int of_wg = p.nt == 0 ? 16 * p.few : 16 * p.waves * p.nt;
         p.tiles = (int)((cols + of_wg - 1) / of_wg);
         const long runs = (p.waves == 4 ? 2L : 1L) * ri_compute_units() / ((long)p.tiles * kv_heads);
         p.pages_per_split = (int)((shared_pages + (runs < 1 ? 1 : runs) - 1) / (runs < 1 ? 1 : runs));
@@ -511,12 +523,17 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     const hipStream_t s = (hipStream_t)stream;
     const unsigned own = (unsigned)of_own, shared = (unsigned)of_shared;
     const dim3 join(heads, tokens);
+#define SH_FEW(DH, ALL, GRID)                                                                           \
+    do {                                                                                                \
+        if (p.few == 1) attn_shared_few_kernel<DH, ALL, 1, 4><<<GRID, 256, 0, s>>>(a);                   \
+        else attn_shared_few_kernel<DH, ALL, 2, 4><<<GRID, 256, 0, s>>>(a);                              \
+    } while (0)
 #define SH_LAUNCH(DH)                                                                                   \
     do {                                                                                                \
         if (p.nt == 0) {                                                                                \
-            if (own + shared) attn_shared_few_kernel<DH, true, 4><<<own + shared, 256, 0, s>>>(a);         \
+            if (own + shared) SH_FEW(DH, true, own + shared);                                           \
         } else {                                                                                        \
-            if (own) attn_shared_few_kernel<DH, false, 4><<<own, 256, 0, s>>>(a);                          \
+            if (own) SH_FEW(DH, false, own);                                                            \
             if (shared == 0) {                                                                          \
             } else if (p.nt == 1) attn_shared_kernel<DH, 1, 4, 2><<<shared, 256, 0, s>>>(a);            \
             else if (p.waves == 4) attn_shared_kernel<DH, 2, 4, 2><<<shared, 256, 0, s>>>(a);           \
@@ -528,6 +545,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     else if (head_dim == 64) SH_LAUNCH(64);
     else SH_LAUNCH(32);
 #undef SH_LAUNCH
+#undef SH_FEW
     RI_LAUNCH_CHECK("attention_shared");
     return 0;
 }
