@@ -1488,8 +1488,9 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     tokens instead of once a sequence.  ``shared`` is a multiple of the page (32 tokens; 0: nothing is shared) and the first
     ``shared / 32`` entries of every row of ``page_table`` are the same pages (the first row's are read).  Any number of new tokens
     a sequence, at most ``max_new`` (one, or a drafted step's few); their keys and values are in the cache.  ``max_len`` bounds every
-    sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  ``q_off`` as in
-    ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
+    sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  What a page holds behind
+    a sequence's last token may be anything; the values of its tokens are finite (a token's weight for a later one is 0, which does
+    not undo an infinity).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
     tokens, stride = qkv.shape
     num_pages, hkv, page_size, dh = k_pages.shape
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -1560,8 +1561,9 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
     """``x @ w.T`` for bfloat16 rows ``x [M, K]`` and a matrix in 4 bits: ``w[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k //
     group])``.  ``codes`` (uint8 ``[N, K / 2]``) hold two neighbouring columns a byte, the even one in the low four bits; ``scales``
     (bfloat16 or float32) and ``zeros`` (uint8; None: 8 everywhere) are ``[N, ceil(K / group)]``.  ``group`` is 32, 64 or a multiple of
-    128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights; more rows
-    go 64 at a time.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at the end."""
+    128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights; with more
+    the codes are read again for every 64.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at
+    the end.  A row of ``x`` with an infinity or NaN gives NaN, the other rows what they gave."""
     if x.dim() != 2 or codes.dim() != 2:
         raise ShapeError(f"x and codes are matrices, got {list(x.shape)} and {list(codes.shape)}")
     (m, k), n = x.shape, codes.shape[0]

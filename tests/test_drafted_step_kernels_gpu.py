@@ -257,6 +257,31 @@ def test_attention_over_shared_pages_reads_its_columns_and_leaves_rows_behind_th
     c.check(got)
 
 
+@pytest.mark.parametrize("heads", [4, 40])
+def test_attention_over_shared_pages_keeps_what_pads_a_batch_to_itself(ops, heads):
+    """Rows that are no sequence's hold NaN at positions that are none; the others are what they are without them."""
+    c = SharedCase([(2, 10), (1, 35)], 96, heads, 2, 64, pad_rows=3, seed=8)
+    c.qkv[3:] = float("nan")
+    c.pos[3:] = [-1, -7, 10 ** 9]
+    got = f64(c.run(ops))
+    assert (got[3:] == 0).all()
+    c.check(torch.tensor(got))
+
+
+@pytest.mark.parametrize("rows, n", [(3, 40), (20, 40), (16, 9000)])
+def test_products_in_4_bits_keep_an_infinity_to_its_row(ops, rows, n):
+    if EMULATED:
+        n = 40
+    x, code, packed, scales, zero = int4_inputs(rows, n, 512, 64, True, torch.bfloat16, False, 4)
+    args = guarded(packed), guarded(scales), 64, guarded(zero), torch.float32
+    want = f64(ops.gemm_int4_bf16(guarded(x), *args))
+    x[1, 70], x[2, 9] = float("inf"), float("nan")
+    got = f64(ops.gemm_int4_bf16(guarded(x), *args))
+    others = np.arange(rows) > 2
+    others[0] = True
+    assert np.array_equal(got[others], want[others]) and not np.isfinite(got[1:3]).any()
+
+
 def test_attention_over_shared_pages_of_tokens_within_them(ops):
     """A token whose position lies among the shared tokens sees the keys up to its own."""
     c = SharedCase([(1, 5), (2, 40)], 96, 4, 2, 64, seed=4)
@@ -540,6 +565,22 @@ def test_drafts_are_refused_where_an_operand_does_not_fit(ops):
 
 
 # ---------------------------------------------------------------- devices, streams, graphs, together
+@pytest.mark.skipif(EMULATED, reason="two devices")
+def test_operands_on_two_devices_are_refused(ops):
+    from rust_inference_amd.errors import InferenceError
+    x, _, packed, scales, zero = int4_inputs(2, 16, 128, 32, True, torch.bfloat16, False)
+    c = SharedCase([(1, 5)], 64, 4, 2, 64)
+    logits, draft, tokens, u = drafted([3], 40, 1.0, True)
+    t = lambda a: torch.tensor(a, dtype=torch.float32)  # noqa: E731
+    for call in (lambda: ops.gemm_int4_bf16(x, packed, scales, 32, zero), lambda: ops.gemm_int4_bf16(x.to(DEV), packed.to(DEV), scales, 32),
+                 lambda: ops.gemm_int4_bf16(x.to(DEV), packed.to(DEV), scales.to(DEV), 32, zero), lambda: c.run(ops, k=c.k),
+                 lambda: c.run(ops, qkv=c.qkv), lambda: ops.verify_drafts(t(logits), i32(tokens), i32([0, 3]), t(u).to(DEV), 1.0),
+                 lambda: ops.verify_drafts(t(logits).to(DEV), i32(tokens), i32([0, 3]), t(u), 1.0),
+                 lambda: ops.verify_drafts(t(logits).to(DEV), i32(tokens), i32([0, 3]), t(u).to(DEV), 1.0, t(draft))):
+        with pytest.raises(InferenceError):
+            call()
+
+
 @pytest.mark.skipif(EMULATED, reason="streams and graphs")
 def test_on_another_stream_and_in_two_graphs_that_are_replayed_in_turn(ops):
     """Each operator on a stream of its own, and two captured graphs of all three whose inputs change between the replays: every
