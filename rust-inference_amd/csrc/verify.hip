@@ -183,7 +183,8 @@ __device__ __forceinline__ void place_of_row(const int32_t* __restrict__ cu, int
 }
 
 // A chunk a wavefront, 64 entries a lane: what is done once a wavefront (place, reductions) is a fifth of its instructions so, a
-// third with 32.  The vector unit bounds this pass nearly as the memory does.
+// third with 32.  The vector unit bounds this pass nearly as the memory does (320 rows x 151,936 and 256 of drafts: 65 to 71 us, 5 to
+// 5.4 TB/s).
 template <bool WIDE>
 __global__ __launch_bounds__(RI_WAVE) void verify_stats(ChunkStats* __restrict__ stats, const float* __restrict__ logits,
                                                         const float* __restrict__ draft, const int32_t* __restrict__ cu, int seqs,
@@ -486,7 +487,7 @@ __global__ __launch_bounds__(VER_PICK_THREADS) void verify_pick(int32_t* __restr
     put_out(accepted, out, tokens, cu, seqs, rows, b, r0, r1, end.row, at + place);
 }
 
-// ---- greedy: the best entry of every chunk, then the walk
+// ---- greedy: the best entry of every chunk, then the walk (192 rows x 151,936: 19.5 us, 6 TB/s, and 3.8)
 struct Best { float value; int id; };
 __device__ __forceinline__ Best better(const Best a, const Best b) {
     return b.value > a.value || (b.value == a.value && b.id < a.id) ? b : a;
