@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(W * 64, 2) attn_shared_kernel(const SharedArgs
 }
 
 // A token's runs and chunks joined, a workgroup a (head, token): DH / 4 neighbouring threads read a run's sums of it, 1,024 / DH
-// such groups take the runs in turn and meet in LDS in their order (64 tokens x 32 heads of 128, 32 runs and up to 3 chunks: 9.5 us).
+// such groups take the runs in turn and meet in LDS in their order (64 tokens x 32 heads of 128, 16 runs and up to 3 chunks: 6.2 us).
 // Tokens that are no sequence's get zeros.
 #define SH_JOIN 256
 template <int DH>
@@ -465,11 +465,15 @@ struct SharedPlan { int nt, few, waves, splits, pages_per_split, tiles, own_tile
 // A sequence that brings more than 16 columns takes them 32 a workgroup, with fewer wavefronts a compute unit, so that its own keys are read
 // half as often: 16 sequences of up to 5 tokens of 4 heads a key head, 20 to 900 own keys, 14.0 us (tiles of 16: 15.7).
 // More than 32 columns a key head take the form of many columns: workgroups of four wavefronts with a tile of 64 or, from 65 columns on,
-// 128, two of them a compute unit; from 129 columns on, where a run is longer than SH_SHORT_PAGES, of eight with 256, whose copies
+// 128; from 129 columns on, where a run is longer than SH_SHORT_PAGES, of eight with 256, whose copies
 // have three turns to arrive instead of one.  us with four : eight wavefronts: 32 sequences of 64 heads behind 131,072 tokens (runs of 128
-// pages) 237 : 215, 64 of 32 heads behind 8,192 (8 pages) 78 : 79, 52 tokens of 32 heads behind 4,096 (8 pages) 43 : 47.  Runs of the
-// shared pages: eight wavefronts a compute unit, eight pages a run at least.
+// pages) 237 : 215, 64 of 32 heads behind 8,192 (8 pages) 78 : 79, 52 tokens of 32 heads behind 4,096 (8 pages) 43 : 47.
+// The shared pages are cut into as many runs as give every compute unit a workgroup, of eight pages at least: every run costs its columns'
+// sums, written and read again.  Twice as many, us: 64 sequences of 32 heads behind 8,192 34.4 : 31.7, 24 behind 16,384 31.6 : 28.6, 8
+// behind 32,768 44 : 34.5.  Where workgroups of four wavefronts would walk more than SH_LONG_PAGES two stand beside one another (24 sequences
+// of 32 heads behind 131,072 127 : 123).
 #define SH_SHORT_PAGES 16
+#define SH_LONG_PAGES 128
 static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads) {
     SharedPlan p;
     const int group = heads / kv_heads;
@@ -483,8 +487,11 @@ static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_page
     for (p.waves = cols <= 128 ? 4 : 8;; p.waves = 4) {
         const int of_wg = p.nt == 0 ? 16 * p.few : 16 * p.waves * p.nt;
         p.tiles = (int)((cols + of_wg - 1) / of_wg);
-        const long runs = (p.waves == 4 ? 2L : 1L) * ri_compute_units() / ((long)p.tiles * kv_heads);
-        p.pages_per_split = (int)((shared_pages + (runs < 1 ? 1 : runs) - 1) / (runs < 1 ? 1 : runs));
+        const long items = (long)p.tiles * kv_heads;
+        long runs = ri_compute_units() / items;
+        if (p.waves == 4 && shared_pages > SH_LONG_PAGES * runs) runs = 2L * ri_compute_units() / items;
+        if (runs < 1) runs = 1;
+        p.pages_per_split = (int)((shared_pages + runs - 1) / runs);
         p.pages_per_split += p.pages_per_split & 1;
         if (p.pages_per_split < 8) p.pages_per_split = 8;
         if (p.waves == 4 || p.pages_per_split > SH_SHORT_PAGES) break;
