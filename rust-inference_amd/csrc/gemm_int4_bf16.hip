@@ -556,7 +556,7 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
     RI_REQUIRE(out && x && codes && scales, "gemm_int4: an operand is missing");
     RI_REQUIRE((uintptr_t)x % 16 == 0, "gemm_int4: x must start on a 16-byte boundary");
     RI_REQUIRE((uintptr_t)codes % 4 == 0, "gemm_int4: the codes must start on a 4-byte boundary");
-    const int groups = (k + group - 1) / group;
+    const int groups = (k - 1) / group + 1;                   // (k + group may pass 32 bits)
     const I4Args a = {out, (const bf16_t*)x, (const uint8_t*)codes, scales, (const uint8_t*)zeros, rows, n, k, groups,
                       group >= 128 ? group / 128 : 1, out_dtype == RI_F32};
     const bool f = scale_dtype == RI_F32;

@@ -1572,6 +1572,7 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
     if m < 1 or n < 1 or k < 8 or k % 8:
         raise ShapeError(f"a product of {m} rows, {n} columns and k {k}: at least one each, k a multiple of 8")
     groups = -(-k // group)
+    group = min(group, -(-k // 128) * 128)                    # (a longer one is the same one group, and the kernel's number has 32 bits)
     _on_current_device(x, codes, scales, zeros)
     out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     _call("ri_gemm_int4_bf16", _dev(out, "out"), code(out_dtype), _dev(x, "x", torch.bfloat16), _dev(codes, "codes", torch.uint8, (n, k // 2)),

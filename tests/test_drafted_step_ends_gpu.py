@@ -1,0 +1,29 @@
+"""The operators of a drafted step at the ends of what they accept: lengths, bounds and numbers that an ordinary step does not bring.
+
+As in tests/test_drafted_step_kernels_gpu.py, the same tests run without a GPU, between guard pages, when the environment says
+RI_TEST_KERNELS=emulated; tests/test_drafted_step_ends.py starts that run."""
+import numpy as np
+import pytest
+import torch
+
+from test_drafted_step_kernels_gpu import _guarded_buffers_go_back, f64, guarded, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
+
+
+# ---------------------------------------------------------------- products with a matrix in 4 bits
+@pytest.mark.parametrize("group", [512, 1024, 2 ** 30, 2 ** 31 - 128, 2 ** 31, 2 ** 32 + 128, 2 ** 40])
+def test_products_in_4_bits_take_a_group_longer_than_the_matrix_as_one(ops, group):
+    """One scale and zero point a row, whatever the group's length; whole numbers, so the sums are exact."""
+    x, code, packed, scales, zero = int4_inputs(3, 20, 512, 512, True, torch.bfloat16, True, 3)
+    xd, w, _, _ = plain_int4(x, code, scales, zero, 512)
+    got = ops.gemm_int4_bf16(guarded(x), guarded(packed), guarded(scales), group, guarded(zero), torch.float32)
+    assert np.array_equal(f64(got), xd @ w.T)
+
+
+def test_the_c_entry_counts_groups_in_its_own_range(ops):
+    """The largest group that its argument holds, straight to the C entry."""
+    x, code, packed, scales, zero = int4_inputs(3, 20, 512, 512, True, torch.bfloat16, True, 4)
+    xd, w, _, _ = plain_int4(x, code, scales, zero, 512)
+    x, packed, scales, zero, out = guarded(x), guarded(packed), guarded(scales), guarded(zero), guarded(torch.zeros(3, 20))
+    ops._call("ri_gemm_int4_bf16", out.data_ptr(), 0, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), 1, zero.data_ptr(), 3, 20, 512,
+              2 ** 31 - 128, ops._stream())
+    assert np.array_equal(f64(out), xd @ w.T)
