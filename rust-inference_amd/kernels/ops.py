@@ -291,6 +291,12 @@ def _on_current_device(first: torch.Tensor, *others) -> None:
         raise KernelError(f"the operands lie on {first.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
+def _in_32_bits(what: str, *sizes: int) -> None:
+    """The sizes fit the C interface's numbers (ctypes would cut off what lies above 32 bits without a word)."""
+    if max(sizes) > 0x7FFFFFFF:
+        raise ShapeError(f"{what} of {' x '.join(str(s) for s in sizes)}: at most 2^31 - 1 each")
+
+
 # ---------------------------------------------------------------- row-wise
 GATE_SIGMOID, GATE_SILU = 0, 1
 
@@ -1571,6 +1577,7 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
         raise ShapeError(f"groups of {group} columns: 32, 64 and multiples of 128 are taken")
     if m < 1 or n < 1 or k < 8 or k % 8:
         raise ShapeError(f"a product of {m} rows, {n} columns and k {k}: at least one each, k a multiple of 8")
+    _in_32_bits("a product of rows, columns and k", m, n, k)
     groups = -(-k // group)
     group = min(group, -(-k // 128) * 128)                    # (a longer one is the same one group, and the kernel's number has 32 bits)
     _on_current_device(x, codes, scales, zeros)

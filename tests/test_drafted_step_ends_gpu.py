@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import _guarded_buffers_go_back, f64, guarded, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
+from test_drafted_step_kernels_gpu import EMULATED, _guarded_buffers_go_back, f64, guarded, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -27,3 +27,14 @@ def test_the_c_entry_counts_groups_in_its_own_range(ops):
     ops._call("ri_gemm_int4_bf16", out.data_ptr(), 0, x.data_ptr(), packed.data_ptr(), scales.data_ptr(), 1, zero.data_ptr(), 3, 20, 512,
               2 ** 31 - 128, ops._stream())
     assert np.array_equal(f64(out), xd @ w.T)
+
+
+@pytest.mark.skipif(not EMULATED, reason="gigabytes that only the CPU's lazy memory gives for nothing")
+@pytest.mark.parametrize("rows, n, k", [(1, 1, 2 ** 32 + 128), (1, 2 ** 32 + 16, 8)])
+def test_products_in_4_bits_refuse_sizes_beyond_32_bits(ops, rows, n, k):
+    """Each size's low 32 bits are those of a small product, which is not the one that was asked for."""
+    from rust_inference_amd.errors import ShapeError
+    group = -(-k // 128) * 128
+    codes, scales = torch.empty(n, k // 2, dtype=torch.uint8), torch.empty(n, 1, dtype=torch.bfloat16)
+    with pytest.raises(ShapeError):
+        ops.gemm_int4_bf16(torch.empty(rows, k, dtype=torch.bfloat16), codes, scales, group)
