@@ -556,6 +556,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     seqs, temperature = cu_seqlens.shape[0] - 1, float(temperature)
     if rows < 1 or vocab < 1:
         raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
+    _in_32_bits("logits of rows and a vocabulary", rows, vocab)
     if temperature > 0 and uniform is None:
         raise ShapeError("a temperature above 0 wants uniform numbers, one a row")
     _on_current_device(logits, tokens, cu_seqlens, uniform, draft_logits)

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import EMULATED, _guarded_buffers_go_back, f64, guarded, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
+from test_drafted_step_kernels_gpu import EMULATED, _guarded_buffers_go_back, f64, guarded, i32, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -38,3 +38,13 @@ def test_products_in_4_bits_refuse_sizes_beyond_32_bits(ops, rows, n, k):
     codes, scales = torch.empty(n, k // 2, dtype=torch.uint8), torch.empty(n, 1, dtype=torch.bfloat16)
     with pytest.raises(ShapeError):
         ops.gemm_int4_bf16(torch.empty(rows, k, dtype=torch.bfloat16), codes, scales, group)
+
+
+# ---------------------------------------------------------------- drafted tokens
+@pytest.mark.skipif(not EMULATED, reason="gigabytes that only the CPU's lazy memory gives for nothing")
+@pytest.mark.parametrize("rows, vocab", [(1, 2 ** 32 + 40), (2 ** 32 + 1, 1)])
+def test_drafts_with_sizes_beyond_32_bits_are_refused(ops, rows, vocab):
+    from rust_inference_amd.errors import ShapeError
+    logits, tokens = torch.empty(rows, vocab), torch.empty(rows, dtype=torch.int32)
+    with pytest.raises(ShapeError):
+        ops.verify_drafts(logits, tokens, i32([0, 1]), None, 0.0)
