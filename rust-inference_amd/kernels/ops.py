@@ -1510,16 +1510,21 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
         raise ShapeError(f"attention: {shared} shared tokens are no whole pages of {page_size}")
     if page_table.dim() != 2 or page_table.shape[0] < seqs:
         raise ShapeError(f"page_table is {list(page_table.shape)} for {seqs} sequences")
+    reach = page_table.shape[1] * page_size
+    if shared > reach or not 1 <= max_len <= reach:           # (before the workspace is sized by them)
+        raise ShapeError(f"attention: {shared} shared tokens, sequences of up to {max_len}, tables of {reach}")
+    _in_32_bits("tables of tokens, queries of tokens and columns, pages", reach, tokens, stride, num_pages)
+    max_new = min(int(max_new), tokens)
     _on_current_device(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table)
     args = (_dev(qkv, "qkv", torch.bfloat16) + 2 * int(q_off), stride, _dev(k_pages, "k_pages", torch.bfloat16),
             _dev(v_pages, "v_pages", torch.bfloat16), _dev(cu_seqlens, "cu_seqlens", torch.int32, (seqs + 1,)),
             _dev(tok_pos, "tok_pos", torch.int32, (tokens,)), _dev(page_table, "page_table", torch.int32))
     first = shared // page_size
-    slots = _get("ri_attention_shared_slots")(tokens, seqs, int(max_new), first, int(max_len), heads, kv_heads)
+    slots = _get("ri_attention_shared_slots")(tokens, seqs, max_new, first, int(max_len), heads, kv_heads)
     ws = torch.empty((max(slots, 1) * tokens * heads * (head_dim + 2),), dtype=torch.float32, device=qkv.device)
     out = torch.empty((tokens, heads * head_dim), dtype=torch.bfloat16, device=qkv.device)
     _call("ri_attention_shared_bf16", _dev(out, "out"), _dev(ws, "workspace"), *args, page_table.shape[1], num_pages, tokens, seqs,
-          int(max_new), first, int(max_len), heads, kv_heads, head_dim, page_size, float(scale), _stream())
+          max_new, first, int(max_len), heads, kv_heads, head_dim, page_size, float(scale), _stream())
     return out
 
 

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import EMULATED, _guarded_buffers_go_back, f64, guarded, i32, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
+from test_drafted_step_kernels_gpu import EMULATED, SharedCase, _guarded_buffers_go_back, f64, guarded, i32, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -38,6 +38,37 @@ def test_products_in_4_bits_refuse_sizes_beyond_32_bits(ops, rows, n, k):
     codes, scales = torch.empty(n, k // 2, dtype=torch.uint8), torch.empty(n, 1, dtype=torch.bfloat16)
     with pytest.raises(ShapeError):
         ops.gemm_int4_bf16(torch.empty(rows, k, dtype=torch.bfloat16), codes, scales, group)
+
+
+# ---------------------------------------------------------------- attention over pages that the batch shares
+@pytest.mark.parametrize("change", [dict(max_len=2 ** 32 + 100), dict(max_len=2 ** 40), dict(shared=2 ** 37 + 64), dict(shared=2 ** 40)])
+def test_attention_over_shared_pages_refuses_lengths_that_no_table_holds(ops, change):
+    """Among them such whose low 32 bits, or whose pages' low 32 bits, are those of the case."""
+    from rust_inference_amd.errors import ShapeError
+    c = SharedCase([(1, 36)], 64, 4, 2, 64)
+    with pytest.raises(ShapeError):
+        c.run(ops, **change)
+
+
+def test_attention_over_shared_pages_allocates_nothing_for_a_length_that_it_refuses(ops, monkeypatch):
+    from rust_inference_amd.errors import ShapeError
+    c = SharedCase([(1, 36)], 64, 4, 2, 64)
+    class Torch:
+        def __getattr__(self, name):
+            assert name != "empty"
+            return getattr(torch, name)
+    args = dict(k=guarded(c.k), v=guarded(c.v), qkv=guarded(c.qkv))
+    monkeypatch.setattr(ops, "torch", Torch())
+    for max_len in (0, -1, 32 * c.width + 1, 2 ** 31 - 1):
+        with pytest.raises(ShapeError):
+            c.run(ops, max_len=max_len, **args)
+
+
+def test_attention_over_shared_pages_takes_any_bound_of_the_new_tokens(ops):
+    """Far above the tokens that there are, its low 32 bits 0 or small."""
+    c = SharedCase([(3, 40), (1, 9)], 64, 4, 2, 64, seed=2)
+    for c.max_new in (3, 100, 2 ** 31 - 1, 2 ** 32, 2 ** 32 + 1):
+        c.check(c.run(ops))
 
 
 # ---------------------------------------------------------------- drafted tokens
