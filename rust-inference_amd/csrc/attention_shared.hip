@@ -481,9 +481,9 @@ static SharedPlan shared_plan(int tokens, int seqs, int max_new, int shared_page
     p.nt = cols <= 32 ? 0 : cols <= 64 ? 1 : 2;
     p.few = (long)max_new * group <= 16 ? 1 : 2;
     p.own_tiles = (int)(((long)max_new * group + 16 * p.few - 1) / (16 * p.few));
-    const int own = max_len - shared_pages * PAGE;
+    const long own = max_len - (long)shared_pages * PAGE;
     p.own_pages = (long)seqs * kv_heads * p.own_tiles <= ri_compute_units() ? SH_OWN_PAGES / 2 : SH_OWN_PAGES;      // (max_len changes no sum)
-    p.own_chunks = own > 0 ? (own + p.own_pages * PAGE - 1) / (p.own_pages * PAGE) : 0;
+    p.own_chunks = own > 0 ? (int)((own + p.own_pages * PAGE - 1) / (p.own_pages * PAGE)) : 0;
     for (p.waves = cols <= 128 ? 4 : 8;; p.waves = 4) {
         const int of_wg = p.nt == 0 ? 16 * p.few : 16 * p.waves * p.nt;
         p.tiles = (int)((cols + of_wg - 1) / of_wg);
@@ -519,7 +519,8 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE(shared_pages >= 0 && shared_pages <= table_width, "attention_shared: %d shared pages, tables of %d", shared_pages, table_width);
     RI_REQUIRE(max_len >= 1 && max_len <= (long)table_width * PAGE, "attention_shared: sequences of up to %d tokens, tables of %d pages", max_len, table_width);
     RI_REQUIRE(kv_heads <= 65535 && tokens <= 65535 && heads <= 65535, "attention_shared: %d tokens, %d heads exceed one launch", tokens, heads);
-    RI_REQUIRE((long)table_width * PAGE < 0x7fffffff, "attention_shared: page table width %d", table_width);
+    // (a token's own keys and a chunk of them are added up in 32 bits)
+    RI_REQUIRE((long)table_width * PAGE <= 0x7fffffff - SH_OWN_PAGES * PAGE, "attention_shared: page table width %d", table_width);
     RI_REQUIRE(scale > 0.f && scale <= FLT_MAX, "attention_shared: scale %g is no positive number", (double)scale);
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
     const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);

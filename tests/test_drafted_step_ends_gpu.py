@@ -71,6 +71,18 @@ def test_attention_over_shared_pages_takes_any_bound_of_the_new_tokens(ops):
         c.check(c.run(ops))
 
 
+def test_attention_over_shared_pages_refuses_lengths_whose_chunks_pass_32_bits(ops):
+    """The widest tables, and lengths within a chunk of 2^31: the count of own chunks is taken in 64 bits, and refused."""
+    from rust_inference_amd.errors import KernelError
+    c = SharedCase([(1, 36)], 64, 4, 2, 64)
+    for width, max_len in ((2 ** 26 - 1, 2 ** 31 - 40), (2 ** 26 - 1, 2 ** 31 - 200), (2 ** 26 - 17, 2 ** 31 - 16 * 32 - 40)):
+        c.table = torch.zeros(1, width, dtype=torch.int32)
+        with pytest.raises(KernelError):
+            c.run(ops, max_len=max_len)
+    assert ops._get("ri_attention_shared_slots")(1, 1, 1, 0, 2 ** 31 - 1, 4, 2) == 2 ** 23
+    assert ops._get("ri_attention_shared_slots")(1, 1, 1, 2 ** 27, 100, 4, 2) > 0
+
+
 # ---------------------------------------------------------------- drafted tokens
 @pytest.mark.skipif(not EMULATED, reason="gigabytes that only the CPU's lazy memory gives for nothing")
 @pytest.mark.parametrize("rows, vocab", [(1, 2 ** 32 + 40), (2 ** 32 + 1, 1)])
