@@ -515,6 +515,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE(head_dim == 32 || head_dim == 64 || head_dim == 128, "attention_shared: head_dim %d (this kernel is built for 32, 64 and 128)", head_dim);
     RI_REQUIRE(page_size == PAGE, "attention_shared: pages of %d tokens (this kernel takes %d)", page_size, PAGE);
     RI_REQUIRE(q_stride >= heads * head_dim && q_stride % 8 == 0 && (uintptr_t)q % 16 == 0, "attention_shared: q row stride %d, or q off a 16-byte boundary", q_stride);
+    RI_REQUIRE((uintptr_t)k_pages % 16 == 0 && (uintptr_t)v_pages % 16 == 0, "attention_shared: pages off a 16-byte boundary");
     RI_REQUIRE(table_width > 0 && num_pages > 0, "attention_shared: page table width %d, %d pages", table_width, num_pages);
     RI_REQUIRE(shared_pages >= 0 && shared_pages <= table_width, "attention_shared: %d shared pages, tables of %d", shared_pages, table_width);
     RI_REQUIRE(max_len >= 1 && max_len <= (long)table_width * PAGE, "attention_shared: sequences of up to %d tokens, tables of %d pages", max_len, table_width);

@@ -83,6 +83,16 @@ def test_attention_over_shared_pages_refuses_lengths_whose_chunks_pass_32_bits(o
     assert ops._get("ri_attention_shared_slots")(1, 1, 1, 2 ** 27, 100, 4, 2) > 0
 
 
+@pytest.mark.parametrize("which", ["k", "v", "qkv"])
+def test_attention_over_shared_pages_refuses_what_does_not_start_on_16_bytes(ops, which):
+    from rust_inference_amd.errors import KernelError
+    c = SharedCase([(1, 36)], 64, 4, 2, 64)
+    t = getattr(c, which)
+    off = guarded(torch.zeros(t.numel() + 8, dtype=torch.bfloat16))[1:1 + t.numel()].view(t.shape)
+    with pytest.raises(KernelError):
+        c.run(ops, **{which: off})
+
+
 # ---------------------------------------------------------------- drafted tokens
 @pytest.mark.skipif(not EMULATED, reason="gigabytes that only the CPU's lazy memory gives for nothing")
 @pytest.mark.parametrize("rows, vocab", [(1, 2 ** 32 + 40), (2 ** 32 + 1, 1)])
