@@ -615,7 +615,7 @@ int ri_branch_norm_add_norm(float* residual, void* act, int act_dtype, const voi
 int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const void* codes, const void* scales, int scale_dtype,
                       const void* zeros, int rows, int n, int k, int group, void* stream);
 
-// Attention of the new tokens of `seqs` sequences (cu_seqlens, at most max_new each) whose page tables begin with the same
+// Attention of the new tokens of `seqs` sequences (cu_seqlens; max_new each sizes the grid) whose page tables begin with the same
 // shared_pages pages (read from the first row of page_table); bfloat16, pages of 32, every sequence at most max_len tokens long after
 // the step.  workspace: ri_attention_shared_slots(...) * tokens * heads * (head_dim + 2) floats.  Tokens that are no sequence's
 // (before cu_seqlens[0], from cu_seqlens[seqs] on) get zeros.

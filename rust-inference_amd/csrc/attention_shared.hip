@@ -86,9 +86,9 @@ __device__ __forceinline__ int first_ids(const int32_t* table, int page0, int pa
 // (own keys of 64 sequences, 204 MB: 39 us, 5.2 TB/s), a short chunk by its chain of loads: place, keys, values.
 template <int DH, int NT, int W, int SLOTS>
 __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W, SLOTS>& lds, const int32_t* table, int kvh, int slot,
-                                            int first_token, int col0, int cols, int page0, int page1, int last_key, int ids) {
+                                            int first_token, int col0, int cols, int page0, int page1, int last_key, int ids, int thread) {
     constexpr int LD = SharedLds<DH, W, SLOTS>::LD;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
+    const int lane = thread & 63, wave = __builtin_amdgcn_readfirstlane(thread >> 6), i = lane & 15, jg = lane >> 4;
     Columns<DH, NT> c;
     init_columns<DH, NT>(c);
     Place place[NT];
@@ -176,7 +176,7 @@ __device__ __forceinline__ void few_columns(const SharedArgs& a, SharedLds<DH, W
                 make_float4(c.o[n][dt][0] * mine, c.o[n][dt][1] * mine, c.o[n][dt][2] * mine, c.o[n][dt][3] * mine);
         if (wave == 0 && jg == 0 && col0 + 16 * n + i < cols) a.stats[result_at(a, slot, place[n])] = make_float2(m, l);
         __syncthreads();
-        for (int at = threadIdx.x; at < 16 * DH / 4; at += W * 64) {
+        for (int at = thread; at < 16 * DH / 4; at += W * 64) {
             const int r = at / (DH / 4), d = at % (DH / 4) * 4, col = col0 + 16 * n + r;
             if (col >= cols) break;
             float4 o = *reinterpret_cast<const float4*>(&meet.o[0][r * LD + d]);
@@ -373,7 +373,14 @@ __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 
     const int last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
     const int page1 = min(page0 + a.own_pages, last_key / PAGE + 1);
     if (page0 >= page1) return;
-    few_columns<DH, NT>(a, lds, table, kvh, a.splits + chunk, first, tile * 16 * NT, cols, page0, page1, last_key, ids);
+    // One tile, unless the sequence brings more tokens than max_new said.  (The compiler is not to know that a thread has the same number in
+    // every turn: what it would keep from one to the next does not fit the registers.)
+    for (int col0 = tile * 16 * NT; col0 < cols; col0 += a.own_tiles * 16 * NT) {
+        int thread = threadIdx.x;
+        ma_here(thread);
+        few_columns<DH, NT>(a, lds, table, kvh, a.splits + chunk, first, col0, cols, page0, page1, last_key, ids, thread);
+        __syncthreads();
+    }
 }
 
 // Few columns in all: the runs of the shared pages and the sequences' own chunks, a workgroup each; with more (ALL false) the own
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(W * 64, NT == 1 ? 3 : 2) attn_shared_few_kerne
     const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads, page0 = slot * a.pages_per_split;
     few_columns<DH, NT>(a, lds, a.page_table, kvh, slot, 0, tile * 16 * NT, a.tokens * (a.heads / a.kv_heads), page0,
                     min(page0 + a.pages_per_split, a.shared_pages), a.shared_pages * PAGE - 1,
-                    first_ids<W>(a.page_table, page0, a.shared_pages));
+                    first_ids<W>(a.page_table, page0, a.shared_pages), threadIdx.x);
 }
 
 // The shared pages' runs for many columns; by rising number a tile after the other, so that tiles that read the same pages lie a multiple

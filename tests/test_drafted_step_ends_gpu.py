@@ -83,6 +83,15 @@ def test_attention_over_shared_pages_refuses_lengths_whose_chunks_pass_32_bits(o
     assert ops._get("ri_attention_shared_slots")(1, 1, 1, 2 ** 27, 100, 4, 2) > 0
 
 
+@pytest.mark.parametrize("lens, shared, heads, kv, dim", [([(20, 40), (1, 30)], 64, 4, 2, 64), ([(9, 700), (3, 3), (30, 33)], 32, 8, 1, 32),
+                                                          ([(17, 18)], 0, 16, 4, 128), ([(6, 6), (0, 0), (40, 600)], 320, 2, 2, 128)])
+def test_attention_over_shared_pages_answers_sequences_that_bring_more_than_the_bound(ops, lens, shared, heads, kv, dim):
+    """max_new sizes the grid; a sequence above it takes longer and gets what it asked for."""
+    c = SharedCase(lens, shared, heads, kv, dim, seed=11)
+    for c.max_new in (1, 4, c.max_new):
+        c.check(c.run(ops))
+
+
 @pytest.mark.parametrize("which", ["k", "v", "qkv"])
 def test_attention_over_shared_pages_refuses_what_does_not_start_on_16_bytes(ops, which):
     from rust_inference_amd.errors import KernelError
