@@ -356,6 +356,14 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
     }
 }
 
+// The largest position of a sequence's new tokens, which as a rule is the last one's; a lane a token.
+__device__ __forceinline__ int last_position(const SharedArgs& a, int first, int behind) {
+    int last = a.tok_pos[min(first + (int)(threadIdx.x & 63), behind - 1)];
+    for (int at = first + 64; at < behind; at += 64) last = max(last, a.tok_pos[min(at + (int)(threadIdx.x & 63), behind - 1)]);
+    for (int m = 1; m < min(behind - first, 64); m *= 2) last = max(last, __shfl_xor(last, m, 64));
+    return __builtin_amdgcn_readfirstlane(last);
+}
+
 // A sequence's own chunk, by its number among all (key heads fastest, then tiles, chunks, sequences).
 template <int DH, int NT, int W>
 __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 0>& lds, int item) {
@@ -370,7 +378,7 @@ __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 
     const int first = min(max(a.cu_seqlens[seq], 0), a.tokens), behind = min(max(a.cu_seqlens[seq + 1], first), a.tokens);
     const int cols = (behind - first) * (a.heads / a.kv_heads);
     if (tile * 16 * NT >= cols) return;
-    const int last_key = min(a.tok_pos[behind - 1], a.table_width * PAGE - 1);
+    const int last_key = min(last_position(a, first, behind), a.table_width * PAGE - 1);
     const int page1 = min(page0 + a.own_pages, last_key / PAGE + 1);
     if (page0 >= page1) return;
     // One tile, unless the sequence brings more tokens than max_new said.  (The compiler is not to know that a thread has the same number in

@@ -1494,8 +1494,8 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     ``attention_prefill_bf16`` and ``attention_decode_bf16`` compute without a window, with the shared pages read once for all new
     tokens instead of once a sequence.  ``shared`` is a multiple of the page (32 tokens; 0: nothing is shared) and the first
     ``shared / 32`` entries of every row of ``page_table`` are the same pages (the first row's are read).  Any number of new tokens
-    a sequence, as a rule at most ``max_new`` (one, or a drafted step's few; it sizes the grid, a sequence that brings more takes longer); their
-    keys and values are in the cache.  ``max_len`` bounds every sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  What a page holds behind
+    a sequence, as a rule at most ``max_new`` (one, or a drafted step's few; it sizes the grid, a sequence that brings more takes longer), their
+    positions in any order; their keys and values are in the cache.  ``max_len`` bounds every sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  What a page holds behind
     a sequence's last token may be anything; the values of its tokens are finite (a token's weight for a later one is 0, which does
     not undo an infinity).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
     tokens, stride = qkv.shape

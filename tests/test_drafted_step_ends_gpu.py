@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import EMULATED, SharedCase, _guarded_buffers_go_back, f64, guarded, i32, int4_inputs, ops, plain_int4, pytestmark  # noqa: F401
+from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, PAGE, SharedCase, _guarded_buffers_go_back, f64, guarded, i32,  # noqa: F401
+                                           int4_inputs, ops, plain_int4, pytestmark)
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -90,6 +91,30 @@ def test_attention_over_shared_pages_answers_sequences_that_bring_more_than_the_
     c = SharedCase(lens, shared, heads, kv, dim, seed=11)
     for c.max_new in (1, 4, c.max_new):
         c.check(c.run(ops))
+
+
+@pytest.mark.parametrize("heads, kv, dim", [(4, 2, 64), (16, 1, 32), (8, 2, 128)])
+def test_attention_over_shared_pages_takes_a_sequences_tokens_in_any_order(ops, heads, kv, dim):
+    """The positions of a sequence fall, repeat or jump; every token sees the keys up to its own, chunks beyond the last token's among them."""
+    c = SharedCase([(3, 1400), (1, 30), (70, 600), (5, 300)], 64, heads, kv, dim, seed=12)
+    rng = np.random.default_rng(12)
+    c.pos[:3] = [64 + 1399, 64 + 2, 64 + 700]
+    c.pos[4:74] = (64 + rng.permutation(np.r_[599, rng.integers(0, 599, 69)])).tolist()
+    c.pos[74:] = [64 + 299, 64 + 299, 10, 64, 63]
+    q, k, v = c.qkv[:, :heads * dim].double().view(-1, heads, dim).numpy(), c.k.double(), c.v.double()
+    got, per, seq = f64(c.run(ops)), heads // kv, np.repeat(np.arange(4), c.counts)
+    assert np.isfinite(got).all()
+    for t, p in enumerate(c.pos):
+        pages = c.table[seq[t], :p // PAGE + 1].long()
+        for h in range(heads):
+            keys = k[pages, h // per].reshape(-1, dim)[:p + 1].numpy()
+            values = v[pages, h // per].transpose(1, 2).reshape(-1, dim)[:p + 1].numpy()
+            s = keys @ q[t, h] * c.scale
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            want, size = w @ values, w @ np.abs(values)
+            # (the weights and the result rounded to bfloat16 once each; float32 scores, as SharedCase.check derives)
+            assert (np.abs(got[t, h * dim:(h + 1) * dim] - want) <= BF16_STEP * np.abs(want) + (BF16_STEP + 2.0 ** -14) * size).all(), (t, h)
 
 
 @pytest.mark.parametrize("which", ["k", "v", "qkv"])
