@@ -80,7 +80,8 @@ def test_attention_over_shared_pages_refuses_lengths_whose_chunks_pass_32_bits(o
         c.table = torch.zeros(1, width, dtype=torch.int32)
         with pytest.raises(KernelError):
             c.run(ops, max_len=max_len)
-    assert ops._get("ri_attention_shared_slots")(1, 1, 1, 0, 2 ** 31 - 1, 4, 2) == 2 ** 23
+    # (chunks of eight pages or, on a machine with fewer compute units than the sequence has key heads, sixteen)
+    assert ops._get("ri_attention_shared_slots")(1, 1, 1, 0, 2 ** 31 - 1, 4, 2) in (2 ** 22, 2 ** 23)
     assert ops._get("ri_attention_shared_slots")(1, 1, 1, 2 ** 27, 100, 4, 2) > 0
 
 
