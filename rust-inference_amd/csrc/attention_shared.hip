@@ -29,6 +29,7 @@ struct SharedArgs {
     const int32_t* tok_pos;
     const int32_t* page_table;
     int q_stride, table_width, num_pages, tokens, seqs, heads, kv_heads, shared_pages;
+    int max_len;                 // of any sequence: keys from there on are not seen
     int splits, pages_per_split, tiles, own_tiles, own_chunks, own_pages;
     float scale_log2;
 };
@@ -200,7 +201,7 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
     typedef CopiedPage<DH> Copied;
     constexpr int HALVES = 8 / W, MINE = HALVES * Copied::MINE;         // half pages, and copies, of a wavefront for a pair
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, jg = lane >> 4;
-    const int last_key = page1 * PAGE - 1, u_last = (page1 - page0 - 1) / 2;
+    const int last_key = min(page1 * PAGE, a.max_len) - 1, u_last = (page1 - page0 - 1) / 2;
     auto& k_lds = lds.pages.k;
     auto& v_lds = lds.pages.v;
     int ids = a.page_table[min(page0 + lane, page1 - 1)];
@@ -217,7 +218,7 @@ __device__ __forceinline__ void many_columns(const SharedArgs& a, SharedLds<DH, 
 #pragma unroll
         for (int ks = 0; ks < DH / 32; ++ks) c.q[j][ks].u = *reinterpret_cast<const uint4*>(q + 32 * ks);
     }
-    const bool all_seen = !__any(min_qpos < last_key);
+    const bool all_seen = !__any(min_qpos < page1 * PAGE - 1);
     // the queries are here before the first copy starts: a wait for them behind it would be one for all copies
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -378,7 +379,7 @@ __device__ __forceinline__ void own_chunk(const SharedArgs& a, SharedLds<DH, W, 
     const int first = min(max(a.cu_seqlens[seq], 0), a.tokens), behind = min(max(a.cu_seqlens[seq + 1], first), a.tokens);
     const int cols = (behind - first) * (a.heads / a.kv_heads);
     if (tile * 16 * NT >= cols) return;
-    const int last_key = min(last_position(a, first, behind), a.table_width * PAGE - 1);
+    const int last_key = min(last_position(a, first, behind), a.max_len - 1);
     const int page1 = min(page0 + a.own_pages, last_key / PAGE + 1);
     if (page0 >= page1) return;
     // One tile, unless the sequence brings more tokens than max_new said.  (The compiler is not to know that a thread has the same number in
@@ -406,7 +407,7 @@ __global__ void __launch_bounds__(W * 64, NT == 1 ? 3 : 2) attn_shared_few_kerne
     item -= tile * of_tile;
     const int slot = item / a.kv_heads, kvh = item - slot * a.kv_heads, page0 = slot * a.pages_per_split;
     few_columns<DH, NT>(a, lds, a.page_table, kvh, slot, 0, tile * 16 * NT, a.tokens * (a.heads / a.kv_heads), page0,
-                    min(page0 + a.pages_per_split, a.shared_pages), a.shared_pages * PAGE - 1,
+                    min(page0 + a.pages_per_split, a.shared_pages), min(a.shared_pages * PAGE, a.max_len) - 1,
                     first_ids<W>(a.page_table, page0, a.shared_pages), threadIdx.x);
 }
 
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(SH_JOIN) attn_shared_join_kernel(bf16_t* __res
         if (group == 0) *to = uint2{0u, 0u};
         return;
     }
-    const int own = min(a.tok_pos[token], a.table_width * PAGE - 1) + 1 - a.shared_pages * PAGE;      // own keys that it sees
+    const int own = min(a.tok_pos[token], a.max_len - 1) + 1 - a.shared_pages * PAGE;      // own keys that it sees
     const int chunks = own > 0 ? min((own + a.own_pages * PAGE - 1) / (a.own_pages * PAGE), a.own_chunks) : 0;
     const int slots = a.splits + chunks;
     const size_t at = (size_t)token * a.heads + head, step = (size_t)a.tokens * a.heads;
@@ -545,7 +546,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     const size_t rows = (size_t)(p.splits + p.own_chunks) * tokens * heads;
     const SharedArgs a = {(float*)workspace, (float2*)((float*)workspace + rows * head_dim), (const bf16_t*)q, (const bf16_t*)k_pages,
                           (const bf16_t*)v_pages, cu_seqlens, tok_pos, page_table, q_stride, table_width, num_pages, tokens, seqs, heads,
-                          kv_heads, shared_pages, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks, p.own_pages,
+                          kv_heads, shared_pages, max_len, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks, p.own_pages,
                           scale * 1.44269504088896341f};
     const hipStream_t s = (hipStream_t)stream;
     const unsigned own = (unsigned)of_own, shared = (unsigned)of_shared;

@@ -118,6 +118,16 @@ def test_attention_over_shared_pages_takes_a_sequences_tokens_in_any_order(ops, 
             assert (np.abs(got[t, h * dim:(h + 1) * dim] - want) <= BF16_STEP * np.abs(want) + (BF16_STEP + 2.0 ** -14) * size).all(), (t, h)
 
 
+@pytest.mark.parametrize("heads, kv, dim", [(4, 2, 64), (16, 1, 32), (40, 2, 128)])
+@pytest.mark.parametrize("max_len", [1, 31, 33, 160, 161, 192, 193, 350, 900, 1161])
+def test_attention_over_shared_pages_sees_no_key_behind_the_bound(ops, heads, kv, dim, max_len):
+    """What lies at max_len and behind it, shared or own, within a page, a chunk or a run, is as if a token's position came before it."""
+    c = SharedCase([(1, 1000), (3, 40), (2, 600)], 160, heads, kv, dim, seed=13)
+    got = c.run(ops, max_len=max_len)
+    c.pos = [min(p, max_len - 1) for p in c.pos]
+    c.check(got)
+
+
 @pytest.mark.parametrize("which", ["k", "v", "qkv"])
 def test_attention_over_shared_pages_refuses_what_does_not_start_on_16_bytes(ops, which):
     from rust_inference_amd.errors import KernelError
