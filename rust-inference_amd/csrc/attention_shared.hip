@@ -538,7 +538,8 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     RI_REQUIRE(kv_heads <= 65535 && tokens <= 65535 && heads <= 65535, "attention_shared: %d tokens, %d heads exceed one launch", tokens, heads);
     // (a token's own keys and a chunk of them are added up in 32 bits)
     RI_REQUIRE((long)table_width * PAGE <= 0x7fffffff - SH_OWN_PAGES * PAGE, "attention_shared: page table width %d", table_width);
-    RI_REQUIRE(scale > 0.f && scale <= FLT_MAX, "attention_shared: scale %g is no positive number", (double)scale);
+    const float scale_log2 = scale * 1.44269504088896341f;
+    RI_REQUIRE(scale > 0.f && scale_log2 <= FLT_MAX, "attention_shared: scale %g is not positive, or log2(e) times it no number", (double)scale);
     RI_REQUIRE(out && workspace && q && k_pages && v_pages && cu_seqlens && tok_pos && page_table, "attention_shared: an operand is missing");
     const SharedPlan p = shared_plan(tokens, seqs, max_new, shared_pages, max_len, heads, kv_heads);
     const long of_shared = (long)p.splits * p.tiles * kv_heads, of_own = (long)p.own_chunks * p.own_tiles * seqs * kv_heads;
@@ -547,7 +548,7 @@ extern "C" int ri_attention_shared_bf16(void* out, void* workspace, const void* 
     const SharedArgs a = {(float*)workspace, (float2*)((float*)workspace + rows * head_dim), (const bf16_t*)q, (const bf16_t*)k_pages,
                           (const bf16_t*)v_pages, cu_seqlens, tok_pos, page_table, q_stride, table_width, num_pages, tokens, seqs, heads,
                           kv_heads, shared_pages, max_len, p.splits, p.pages_per_split, p.tiles, p.own_tiles, p.own_chunks, p.own_pages,
-                          scale * 1.44269504088896341f};
+                          scale_log2};
     const hipStream_t s = (hipStream_t)stream;
     const unsigned own = (unsigned)of_own, shared = (unsigned)of_shared;
     const dim3 join(heads, tokens);

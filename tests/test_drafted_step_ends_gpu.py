@@ -128,6 +128,17 @@ def test_attention_over_shared_pages_sees_no_key_behind_the_bound(ops, heads, kv
     c.check(got)
 
 
+def test_attention_over_shared_pages_refuses_a_scale_that_its_exponents_do_not_hold(ops):
+    """Scores are taken times log2(e); the largest scale that this leaves finite gives every token its best key."""
+    from rust_inference_amd.errors import KernelError
+    c = SharedCase([(1, 36)], 64, 4, 2, 64)
+    for c.scale in (3e38, 2.4e38, float("nan"), -1.0):
+        with pytest.raises(KernelError):
+            c.run(ops)
+    c.scale = 1e36                                            # (64 products of normal numbers below 5: below 1600, 1600 x 1e36 x log2(e) is a float)
+    c.check(c.run(ops))
+
+
 @pytest.mark.parametrize("which", ["k", "v", "qkv"])
 def test_attention_over_shared_pages_refuses_what_does_not_start_on_16_bytes(ops, which):
     from rust_inference_amd.errors import KernelError
