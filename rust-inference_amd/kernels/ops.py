@@ -1497,7 +1497,8 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     a sequence, as a rule at most ``max_new`` (one, or a drafted step's few; it sizes the grid, a sequence that brings more takes longer), their
     positions in any order; their keys and values are in the cache.  ``max_len`` bounds every sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  What a page holds behind
     a sequence's last token may be anything; the values of its tokens are finite (a token's weight for a later one is 0, which does
-    not undo an infinity).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
+    not undo an infinity).  ``scale`` times a query's product with a key stays below 10^9 in magnitude, as in the other matrix-core attentions
+    (a score's float32 exponent against the largest one's has to).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
     tokens, stride = qkv.shape
     num_pages, hkv, page_size, dh = k_pages.shape
     if kv_heads < 1 or heads < 1 or heads % kv_heads:

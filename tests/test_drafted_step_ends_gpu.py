@@ -129,13 +129,21 @@ def test_attention_over_shared_pages_sees_no_key_behind_the_bound(ops, heads, kv
 
 
 def test_attention_over_shared_pages_refuses_a_scale_that_its_exponents_do_not_hold(ops):
-    """Scores are taken times log2(e); the largest scale that this leaves finite gives every token its best key."""
+    """Scores are taken times log2(e)."""
     from rust_inference_amd.errors import KernelError
     c = SharedCase([(1, 36)], 64, 4, 2, 64)
     for c.scale in (3e38, 2.4e38, float("nan"), -1.0):
         with pytest.raises(KernelError):
             c.run(ops)
-    c.scale = 1e36                                            # (64 products of normal numbers below 5: below 1600, 1600 x 1e36 x log2(e) is a float)
+
+
+@pytest.mark.parametrize("heads", [4, 40])
+def test_attention_over_shared_pages_of_scores_up_to_a_billion(ops, heads):
+    """Whole queries and keys up to 8: dot products are exact and at most 4,096, times 2^17 the scores reach 5e8.  The largest score's
+    product with log2(e), below 2^30, is off by at most 2^5, which is the exponent that all weights of a column share."""
+    c = SharedCase([(1, 36), (3, 70)], 192, heads, 2, 64, seed=14)
+    whole = lambda t: torch.where(t.isnan(), t, torch.randint(-8, 9, t.shape, generator=torch.Generator().manual_seed(15)).to(t.dtype))  # noqa: E731
+    c.k, c.qkv, c.scale = whole(c.k), whole(c.qkv), 2.0 ** 17
     c.check(c.run(ops))
 
 
