@@ -537,7 +537,7 @@ __global__ __launch_bounds__(VER_THREADS) void verify_walk(int32_t* __restrict__
             Best best = {-INFINITY, 0};
             for (int c = lane; c < chunks; c += RI_WAVE) best = better(best, bests[(size_t)row * chunks + c]);
             best = wave_best(best);
-            if (row == r1 - 1 || tokens[row + 1] != best.id) ends = best.id;
+            if (row == r1 - 1 || tokens[row + 1] != best.id || best.value == -INFINITY) ends = best.id;      // (a row that masks everything: 0)
         }
         if (lane == 0) tried[wave] = ends;
         __syncthreads();

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, PAGE, SharedCase, _guarded_buffers_go_back, f64, guarded, i32,  # noqa: F401
-                                           int4_inputs, ops, plain_int4, pytestmark)
+                                           int4_inputs, ops, plain_int4, pytestmark, verify)
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -165,3 +165,17 @@ def test_drafts_with_sizes_beyond_32_bits_are_refused(ops, rows, vocab):
     logits, tokens = torch.empty(rows, vocab), torch.empty(rows, dtype=torch.int32)
     with pytest.raises(ShapeError):
         ops.verify_drafts(logits, tokens, i32([0, 1]), None, 0.0)
+
+
+@pytest.mark.parametrize("vocab", [1, 3, 300, 4096, 9000])
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_a_row_that_masks_everything_lets_no_draft_stand(ops, vocab, temperature):
+    """Token 0 among the drafts, which is also the token that such a row gives; a row before it in which 0 is the best lets it stand."""
+    masked = np.full((5, vocab), -np.inf, dtype=np.float32)
+    masked[1::2] = np.nan
+    u = np.zeros(5)
+    accepted, out = verify(ops, masked, None, np.array([0, 0, 0, 0, 0]), [2, 3], u, temperature)
+    assert accepted.tolist() == [0, 0] and out.tolist() == [0, -1, 0, -1, -1]
+    masked[2, 0] = masked[0, vocab - 1] = -3e38
+    accepted, out = verify(ops, masked, None, np.array([0, vocab - 1, 0, 0, 0]), [2, 3], u, temperature)
+    assert accepted.tolist() == [1, 1] and out.tolist() == [vocab - 1, 0, 0, 0, -1]
