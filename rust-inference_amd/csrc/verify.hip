@@ -511,8 +511,10 @@ __global__ __launch_bounds__(VER_THREADS) void verify_best(Best* __restrict__ be
     load_chunk<WIDE>(v, logits + (size_t)row * vocab + at, n);
     Best best = {-INFINITY, at};                              // (a chunk of masked entries names its first)
 #pragma unroll
-    for (int e = 0; e < EACH; ++e)
-        if (v[e] > best.value) best = {v[e], at + place_of<WIDE, EACH>(e)};      // (by rising place; NaN is above nothing)
+    for (int e = 0; e < EACH; ++e) {
+        const float x = __builtin_amdgcn_fmed3f(v[e], -INFINITY, FLT_MAX);      // (an infinity is the largest number; NaN the least of the others)
+        if (x > best.value) best = {x, at + place_of<WIDE, EACH>(e)};            // (by rising place)
+    }
     best = wave_best(best);
     if (lane == 0) shared[wave] = best;
     __syncthreads();

@@ -179,3 +179,19 @@ def test_a_row_that_masks_everything_lets_no_draft_stand(ops, vocab, temperature
     masked[2, 0] = masked[0, vocab - 1] = -3e38
     accepted, out = verify(ops, masked, None, np.array([0, vocab - 1, 0, 0, 0]), [2, 3], u, temperature)
     assert accepted.tolist() == [1, 1] and out.tolist() == [vocab - 1, 0, 0, 0, -1]
+
+
+@pytest.mark.parametrize("vocab", [10, 4096, 9001])
+def test_greedy_takes_an_infinity_for_the_largest_number(ops, vocab):
+    """The first of an infinity and the largest finite number is the best, whichever of them it is, in one chunk or in two; with a
+    temperature both weigh one half."""
+    top = np.finfo(np.float32).max
+    logits = np.zeros((4, vocab), dtype=np.float32)
+    first, second = 3, vocab - 1
+    logits[0, [first, second]], logits[1, [first, second]], logits[2, [first, second]] = (top, np.inf), (np.inf, top), (np.inf, np.inf)
+    logits[3, [first, second]], logits[:, 1], logits[:, 2] = (np.nextafter(top, np.float32(0)), np.inf), np.nan, -np.inf
+    tokens = np.array([0, first, first, first])
+    accepted, out = verify(ops, logits, None, tokens, [4], None, 0.0)
+    assert accepted.tolist() == [3] and out.tolist() == [first, first, first, second]
+    accepted, out = verify(ops, logits[:2], None, tokens[:2], [2], np.array([0.25, 0.75]), 1.0)
+    assert accepted.tolist() == [1] and out.tolist() == [first, second]
