@@ -71,7 +71,8 @@ __device__ __forceinline__ double exp2_nonpositive(double t) {
 // The exponentials of a row's (or a chunk's) entries over that of its largest one.  Ordinary temperatures: with M the whole
 // number next to m s, 2^(x s - M) takes thirteen float64 instructions, since x s + (1.5 * 2^52 - M) has the whole part in
 // place at once, and x is held in float32 to what the exponent has room for: lo, where the result is 2^-1000 up to the
-// rounding of lo.  That wants |M| below 2^27 and lo in float32's range; `plain` does without.  NaN and what lies at lo or below is a masked entry, an
+// rounding of lo, which is that of a normal number (2^-24, some 2^3 exponents) where |M| is below 2^27, lo in float32's range and s below
+// 2^80 (lo, where it is not 0, is a whole number of 1 / s); `plain` does without.  NaN and what lies at lo or below is a masked entry, an
 // infinite logit the largest finite number.
 struct Scale { double s, inv; };                 // log2(e) / T and its inverse
 struct Exps {
@@ -85,7 +86,7 @@ __device__ __forceinline__ Exps exps_below(double m, Scale by) {
     r.s = by.s;
     r.top = (float)m;
     const double lo = (whole - 1000.0) * by.inv;
-    r.plain = !(fabs(whole) < 134217728.0 && lo >= -FLT_MAX);
+    r.plain = !(fabs(whole) < 134217728.0 && lo >= -FLT_MAX && by.s < 1.2089258196146292e24);
     r.c = VER_MAGIC - whole;
     r.lo = (float)lo;
     r.back = r.plain ? 1.0 : exp2_parts(fma(-m, by.s, whole), 0.0);

@@ -195,3 +195,45 @@ def test_greedy_takes_an_infinity_for_the_largest_number(ops, vocab):
     assert accepted.tolist() == [3] and out.tolist() == [first, first, first, second]
     accepted, out = verify(ops, logits[:2], None, tokens[:2], [2], np.array([0.25, 0.75]), 1.0)
     assert accepted.tolist() == [1] and out.tolist() == [first, second]
+
+
+@pytest.mark.parametrize("temperature", [1e-20, 1e-24, 1.1e-24, 1.3e-24, 1e-30, 1e-36, 1e-40, 1e-44, 1e-46, 3e-47, 1e-47, 1e-48, 1e-60, 1e-200, 1e-300, 5e-324])
+@pytest.mark.parametrize("top", [0.0, 1e-38, -1e-38, 1.5, -40.0])
+def test_the_coldest_temperatures(ops, temperature, top):
+    """A largest logit of 0, as where logits are shifted to it, or a small, an ordinary one; entries 2^-149, the least that float32 tells apart,
+    to 2^-126 below it.  Every entry weighs 0, the same as the largest or, at temperatures about that distance, something in between."""
+    vocab, counts = 4200, [3, 3, 2]
+    rng = np.random.default_rng(16)
+    logits = (top - 0.1 - np.abs(rng.standard_normal((8, vocab)))).astype(np.float32)
+    best = rng.integers(0, vocab, 8)
+    logits[np.arange(8), best] = top
+    for r, d in enumerate((1e-45, 3e-45, 1e-43, 1e-40, 1.2e-38, 1e-37, 1e-35, 1e-30)):
+        logits[r, (best[r] + 7) % vocab] = np.float32(np.float64(np.float32(top)) - d)
+    logits[:, 11][best != 11] = -np.inf
+    tokens = np.roll(best, 1)
+    tokens[4] = (best[3] + 7) % vocab                        # the entry a little below the best
+    u = np.full(8, 0.3, dtype=np.float32)
+    near = (logits.astype(np.float64) - logits.max(1, keepdims=True).astype(np.float64))
+    with np.errstate(over="ignore"):
+        p = np.exp(near / temperature)
+    p /= p.sum(1, keepdims=True)
+    accepted, out, at = [], [], 0
+    for n in counts:                                          # looked-up drafts: a draft stands if u < p, else it is taken out
+        stop = next((r for r in range(at, at + n - 1) if not u[r] < p[r, tokens[r + 1]]), at + n - 1)
+        weights = p[stop].copy()
+        if stop < at + n - 1:
+            weights[tokens[stop + 1]] = 0.0
+            if not weights.sum() > 0:
+                weights = p[stop]
+        upto = np.cumsum(weights)
+        target = float(u[at + n - 1]) * upto[-1]
+        # (nothing lies within 1e-9 of a border, far above what an exponential and a sum of two such entries are off by)
+        assert np.abs(upto[weights > 0] - target).min() > 1e-9 * upto[-1] and all(abs(p[r, tokens[r + 1]] - u[r]) > 1e-9 for r in range(at, at + n - 1))
+        accepted.append(stop - at)
+        out += tokens[at + 1:stop + 1].tolist() + [int((upto > target).argmax())] + [-1] * (at + n - 1 - stop)
+        at += n
+    got = verify(ops, logits, None, tokens, counts, u, temperature)
+    assert got[0].tolist() == accepted and got[1].tolist() == out
+    # drafts drawn from the target itself: q = p, and every one that has any weight stands
+    got = verify(ops, logits, np.roll(logits, 1, 0), np.roll(best, 1), counts, u, temperature)
+    assert got[0].tolist() == [n - 1 for n in counts]
