@@ -513,8 +513,8 @@ __global__ __launch_bounds__(VER_THREADS) void verify_best(Best* __restrict__ be
     Best best = {-INFINITY, at};                              // (a chunk of masked entries names its first)
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        const float x = __builtin_amdgcn_fmed3f(v[e], -INFINITY, FLT_MAX);      // (an infinity is the largest number; NaN the least of the others)
-        if (x > best.value) best = {x, at + place_of<WIDE, EACH>(e)};            // (by rising place)
+        const float x = v[e] > FLT_MAX ? FLT_MAX : v[e];      // (an infinity is the largest number; a NaN stays one)
+        if (x > best.value) best = {x, at + place_of<WIDE, EACH>(e)};            // (by rising place; NaN is above nothing)
     }
     best = wave_best(best);
     if (lane == 0) shared[wave] = best;

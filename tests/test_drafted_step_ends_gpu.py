@@ -197,6 +197,18 @@ def test_greedy_takes_an_infinity_for_the_largest_number(ops, vocab):
     assert accepted.tolist() == [1] and out.tolist() == [first, second]
 
 
+@pytest.mark.parametrize("vocab", [7, 4097, 9000])
+def test_greedy_takes_no_nan_for_a_number(ops, vocab):
+    """NaN at the lowest ids, at every other one and everywhere but one."""
+    logits = np.full((3, vocab), np.nan, dtype=np.float32)
+    logits[0, 2:], logits[1, 1::2], logits[2, vocab - 2] = -5.0, -np.inf, -3e38
+    logits[0, 5] = 1.0
+    accepted, out = verify(ops, logits, None, np.array([0, 5, 0]), [3], None, 0.0)
+    assert accepted.tolist() == [1] and out.tolist() == [5, 0, -1]
+    accepted, out = verify(ops, logits[2:], None, np.array([0]), [1], None, 0.0)
+    assert accepted.tolist() == [0] and out.tolist() == [vocab - 2]
+
+
 @pytest.mark.parametrize("temperature", [1e-20, 1e-24, 1.1e-24, 1.3e-24, 1e-30, 1e-36, 1e-40, 1e-44, 1e-46, 3e-47, 1e-47, 1e-48, 1e-60, 1e-200, 1e-300, 5e-324])
 @pytest.mark.parametrize("top", [0.0, 1e-38, -1e-38, 1.5, -40.0])
 def test_the_coldest_temperatures(ops, temperature, top):
