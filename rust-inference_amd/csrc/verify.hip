@@ -184,8 +184,8 @@ __device__ __forceinline__ void place_of_row(const int32_t* __restrict__ cu, int
 }
 
 // A chunk a wavefront, 64 entries a lane: what is done once a wavefront (place, reductions) is a fifth of its instructions so, a
-// third with 32.  The vector unit bounds this pass nearly as the memory does (320 rows x 151,936 and 256 of drafts: 65 to 71 us, 5 to
-// 5.4 TB/s).
+// third with 32.  The vector unit bounds this pass nearly as the memory does (320 rows x 151,936 and 256 of drafts, 350 MB: 69 us, 5.1 TB/s;
+// with the 64 rows of draft logits that are no draft's read too 70.5 on the same machine).
 template <bool WIDE>
 __global__ __launch_bounds__(RI_WAVE) void verify_stats(ChunkStats* __restrict__ stats, const float* __restrict__ logits,
                                                         const float* __restrict__ draft, const int32_t* __restrict__ cu, int seqs,
@@ -195,10 +195,16 @@ __global__ __launch_bounds__(RI_WAVE) void verify_stats(ChunkStats* __restrict__
     const bool of_draft = blockIdx.z == 1;
     const int at = chunk * VER_CHUNK, n = min(VER_CHUNK, vocab - at);
     float v[EACH];
-    load_chunk<WIDE>(v, (of_draft ? draft : logits) + (size_t)row * vocab + at, n);
     bool within, drafted;
-    place_of_row(cu, seqs, rows, row, within, drafted);
-    if (of_draft ? !drafted : !within) return;                // nobody asks about this row
+    if (of_draft) {                                           // (a row of every sequence is no draft's: not read)
+        place_of_row(cu, seqs, rows, row, within, drafted);
+        if (!drafted) return;
+    }
+    load_chunk<WIDE>(v, (of_draft ? draft : logits) + (size_t)row * vocab + at, n);
+    if (!of_draft) {                                          // (nearly every row is a sequence's: read beside the question)
+        place_of_row(cu, seqs, rows, row, within, drafted);
+        if (!within) return;
+    }
     float top = -INFINITY;                                    // (the larger of a number and NaN is the number)
 #pragma unroll
     for (int e = 0; e < EACH; ++e) top = fmaxf(top, v[e]);

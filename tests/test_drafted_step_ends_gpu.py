@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, PAGE, SharedCase, _guarded_buffers_go_back, f64, guarded, i32,  # noqa: F401
+from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, PAGE, SharedCase, _guarded_buffers_go_back, drafted, f64, guarded, i32,  # noqa: F401
                                            int4_inputs, ops, plain_int4, pytestmark, verify)
 
 
@@ -249,3 +249,20 @@ def test_the_coldest_temperatures(ops, temperature, top):
     # drafts drawn from the target itself: q = p, and every one that has any weight stands
     got = verify(ops, logits, np.roll(logits, 1, 0), np.roll(best, 1), counts, u, temperature)
     assert got[0].tolist() == [n - 1 for n in counts]
+
+
+@pytest.mark.skipif(not EMULATED, reason="a row that must not be read lies in a guard page")
+@pytest.mark.parametrize("vocab", [40, 4097])
+def test_draft_logits_of_tokens_that_are_no_drafts_are_not_read(ops, vocab):
+    """The C entry is told of a row before the buffer's first, which is that of a sequence's first token."""
+    import emulated
+    logits, draft, tokens, u = drafted([3], vocab, 1.0, True, 17)
+    held = emulated.tensor(torch.tensor(draft[1:]), "draft logits", flush_end=False)
+    t = lambda a: guarded(torch.tensor(np.ascontiguousarray(a), dtype=torch.float32))  # noqa: E731
+    args, cu, ids = (t(logits), t(u)), i32([0, 3]), i32(tokens)
+    words = ops._get("ri_verify_drafts_workspace_words")(1, 3, vocab, 1)
+    accepted, out, ws = i32([0]), i32([0, 0, 0]), guarded(torch.zeros(words, dtype=torch.float64))
+    ops._call("ri_verify_drafts", accepted.data_ptr(), out.data_ptr(), args[0].data_ptr(), held.data_ptr() - 4 * vocab, ids.data_ptr(), cu.data_ptr(),
+              args[1].data_ptr(), ws.data_ptr(), 1, 3, vocab, 1.0, 0)
+    want = verify(ops, logits, draft, tokens, [3], u, 1.0)
+    assert np.array_equal(accepted.numpy(), want[0]) and np.array_equal(out.numpy(), want[1])
