@@ -7,13 +7,14 @@
 // the four lanes of a row hold, so that step s of the piece has columns 32 s + 8 j .. +7 in lane group j: the operand order of
 // the matrix cores' 16 x 16 x 32 product, with x loaded in the same order.
 //
-// A code c becomes a bfloat16 by three bits of arithmetic: 16.0 has a step of 1/8 in its last place, so 0x4180 | c << 3 is
-// 16 + c, exactly, and two codes that lie 16 bits apart in a word turn in one instruction pair (mask and or after a shift).
-// What that adds, s (16 + z) sum x, goes out again: the sums of x are made of the same operands against ones, and their products
-// with s (16 + z) are a product in float32 over the groups, four of them in an instruction of the matrix cores, whose operand
+// A code c becomes a bfloat16 by three bits of arithmetic: a number from 2^-8 on has a step of 2^-15 in its last place, so 0x3B80 | c << 3
+// is (16 + c) / 4096, exactly, and two codes that lie 16 bits apart in a word turn in one instruction pair (mask and or after a shift).
+// What that adds, s (16 + z) / 4096 sum x, goes out again: the sums of x are made of the same operands against numbers of 1/128, and their
+// products with s (16 + z) / 32 are a product in float32 over the groups, four of them in an instruction of the matrix cores, whose operand
 // order is the order in which the lanes hold what they have loaded of s and z.  All sums are float32; taking off what was added
-// costs the result some three of its 24 bits.  Two codes that neighbour in a word are four columns apart, so x's words are
-// permuted alike.
+// costs the result some three of its 24 bits.  A result is multiplied by 4096 when it is stored: so much smaller no sum over 128 columns
+// leaves float32's range, however large x is (with 16 + c itself x of 3e35 did), and results from 2^-114 on keep all their bits.  Two codes
+// that neighbour in a word are four columns apart, so x's words are permuted alike.
 //
 // The wavefronts of a workgroup share the K pieces in turn and meet in LDS, in order.  A piece's codes (and x, where the
 // registers hold it twice) are asked for while the piece before is worked on; a lane group of four loads the scales and zero points
@@ -86,7 +87,13 @@ __device__ __forceinline__ void turn_words(uint32_t (&w)[4]) {
     w[3] = d.y;
 }
 
-// Eight codes as 16 + c, in the order 0 4 1 5 2 6 3 7 of the word's nibbles.  mask is 0x00780078 and sixteen 0x41804180, held in
+// What a code is smaller by, and its parts: the sums' of x and the zero points'.
+#define I4_BACK 4096.f
+#define I4_SIXTEEN 0x3B803B80u   // two times 16 / 4096
+#define I4_ONES 0x3C003C00u      // two times 1 / 128
+__device__ __forceinline__ float taken_off(float scale, uint8_t zero) { return -scale * fmaf((float)zero, 1.f / 32.f, 16.f / 32.f); }
+
+// Eight codes as (16 + c) / 4096, in the order 0 4 1 5 2 6 3 7 of the word's nibbles.  mask is 0x00780078 and sixteen I4_SIXTEEN, held in
 // registers that the compiler does not see through: an instruction takes one literal, and with two the and and the or would be
 // one each.
 __device__ __forceinline__ void widen(I4Frag& f, uint32_t w, uint32_t mask, uint32_t sixteen) {
@@ -106,7 +113,7 @@ __device__ __forceinline__ void reorder(I4Frag& f, const uint4 u) {
 // acc += a . b of the matrix cores' 16 x 16 x 4 product in float32: lane l holds a[l % 16][l / 16] and b[l / 16][l % 16].
 __device__ __forceinline__ void add_product4(i4_floatx4& acc, float a, float b) { acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0); }
 
-// sum over the 32 STEPS columns of x's fragments from xf on, of row l % 16 in lane l.
+// 1 / 128 of the sum over the 32 STEPS columns of x's fragments from xf on, of row l % 16 in lane l.
 template <int STEPS>
 __device__ __forceinline__ float sum_of(const I4Frag* xf, const I4Frag& ones) {
     i4_floatx4 s = {0.f, 0.f, 0.f, 0.f};
@@ -159,11 +166,11 @@ __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) 
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int t = 0; t < NT; ++t) total[mt][t] = i4_floatx4{0.f, 0.f, 0.f, 0.f};
-    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
+    uint32_t mask = 0x00780078u, sixteen = I4_SIXTEEN;
     ma_opaque(mask);
     ma_here(sixteen);
     I4Frag ones;
-    ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = 0x3F803F80u;
+    ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = I4_ONES;
 
     struct Groups { S scale[NT]; uint8_t zero[NT]; };        // as loaded: a conversion would wait for the load
     // Loads stay out of branches, so that the compiler counts them in flight: one that nobody wants reads what every lane reads.
@@ -193,7 +200,7 @@ __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) 
         for (int t = 0; t < NT; ++t) {
             const float own = to_f32(g.scale[t]);
             to_all(scale[t], own);
-            less[t] = -own * (16.f + (float)g.zero[t]);
+            less[t] = taken_off(own, g.zero[t]);
         }
     };
     // first: which of the four groups the piece meets first
@@ -313,8 +320,9 @@ __global__ __launch_bounds__(W * RI_WAVE) void gemm_int4_kernel(const I4Args a) 
             for (int e = 0; e < 4; ++e) {
                 const int m = m0 + 16 * mt + 4 * j + e;
                 if (m < a.rows && c < a.n) {
-                    if (a.out_f32) ((float*)a.out)[(size_t)m * a.n + c] = total[mt][t][e];
-                    else ((bf16_t*)a.out)[(size_t)m * a.n + c] = f32_to_bf16(total[mt][t][e]);
+                    const float value = total[mt][t][e] * I4_BACK;
+                    if (a.out_f32) ((float*)a.out)[(size_t)m * a.n + c] = value;
+                    else ((bf16_t*)a.out)[(size_t)m * a.n + c] = f32_to_bf16(value);
                 }
             }
         }
@@ -348,12 +356,12 @@ __global__ __launch_bounds__(8 * RI_WAVE, 2) void gemm_int4_rows_kernel(const I4
     const uint8_t* zeros = a.zeros ? a.zeros : i4_zero_point;
     const uint32_t zero_mask = a.zeros ? ~0u : 0u;
 
-    uint32_t mask = 0x00780078u, sixteen = 0x41804180u;
+    uint32_t mask = 0x00780078u, sixteen = I4_SIXTEEN;
     ma_opaque(mask);
     ma_here(sixteen);
     I4Frag ones, xf[PP][4];
     float sum[BLOCKS];                                        // of the groups that lane group j holds
-    ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = 0x3F803F80u;
+    ones.w[0] = ones.w[1] = ones.w[2] = ones.w[3] = I4_ONES;
     const bf16_t* x_row = a.x + (size_t)min(i, a.rows - 1) * a.k;
 #pragma unroll
     for (int p = 0; p < PP; ++p)
@@ -422,7 +430,7 @@ __global__ __launch_bounds__(8 * RI_WAVE, 2) void gemm_int4_rows_kernel(const I4
         for (int b = 0; b < BLOCKS; ++b) {
             const float own = to_f32(t.scale[b]);
             to_all(scale[b], own);
-            add_product4(total, sum[b], -own * (16.f + (float)t.zero[b]));
+            add_product4(total, sum[b], taken_off(own, t.zero[b]));
         }
         I4Frag wf[2][4];
 #pragma unroll
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(8 * RI_WAVE, 2) void gemm_int4_rows_kernel(const I4
             o = make_float4(o.x + more.x, o.y + more.y, o.z + more.z, o.w + more.w);
         }
         const int col = 16 * tile + row_of;
-        const float value[4] = {o.x, o.y, o.z, o.w};
+        const float value[4] = {o.x * I4_BACK, o.y * I4_BACK, o.z * I4_BACK, o.w * I4_BACK};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int m = 4 * j + e;

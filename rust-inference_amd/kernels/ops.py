@@ -1576,7 +1576,8 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
     (bfloat16 or float32) and ``zeros`` (uint8; None: 8 everywhere) are ``[N, ceil(K / group)]``.  ``group`` is 32, 64 or a multiple of
     128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights; with more
     the codes are read again for every 64.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at
-    the end.  A row of ``x`` with an infinity or NaN gives NaN, the other rows what they gave."""
+    the end.  The sums stay in range for any finite ``x`` for which the sum of ``|scale x|`` over ``K`` does; results below 2^-114 in magnitude have
+    fewer bits.  A row of ``x`` with an infinity or NaN gives NaN, the other rows what they gave."""
     if x.dim() != 2 or codes.dim() != 2:
         raise ShapeError(f"x and codes are matrices, got {list(x.shape)} and {list(codes.shape)}")
     (m, k), n = x.shape, codes.shape[0]

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, PAGE, SharedCase, _guarded_buffers_go_back, drafted, f64, guarded, i32,  # noqa: F401
+from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, F32_STEP, PAGE, SharedCase, _guarded_buffers_go_back, drafted, f64, guarded, i32,  # noqa: F401
                                            int4_inputs, ops, plain_int4, pytestmark, verify)
 
 
@@ -39,6 +39,62 @@ def test_products_in_4_bits_refuse_sizes_beyond_32_bits(ops, rows, n, k):
     codes, scales = torch.empty(n, k // 2, dtype=torch.uint8), torch.empty(n, 1, dtype=torch.bfloat16)
     with pytest.raises(ShapeError):
         ops.gemm_int4_bf16(torch.empty(rows, k, dtype=torch.bfloat16), codes, scales, group)
+
+
+FORMS = [  # rows, n, k, group: the forms of a whole machine and, on one of one compute unit, the one that holds x
+    (1, 16, 128, 128), (3, 40, 1160, 64), (17, 48, 264, 32), (45, 50, 200, 64), (65, 18, 416, 32), (16, 200, 2080, 64), (9, 331, 4096, 128),
+    (2, 100, 1408, 384), (130, 16, 128, 64),
+]
+if not EMULATED:
+    FORMS += [(16, 9001, 1056, 64), (8, 16500, 2048, 32), (5, 8210, 4096, 256), (40, 8300, 200, 64), (20, 8200, 640, 128), (49, 33001, 136, 64)]
+
+
+@pytest.mark.parametrize("rows, n, k, group", FORMS)
+@pytest.mark.parametrize("zeros", [True, False])
+@pytest.mark.parametrize("exponent", [100, 112, 125, -60, -100])
+def test_products_in_4_bits_of_very_large_and_very_small_x_are_exact(ops, rows, n, k, group, zeros, exponent):
+    """Whole numbers up to 4 times a power of two, scales of such a power that results stay in range: the same exact products, shifted.  (The
+    largest x, 2^127; the smallest sums are multiples of 2^-3 x 2^-100 x 2^-12, a normal number.)"""
+    x, code, packed, scales, zero = int4_inputs(rows, n, k, group, zeros, torch.float32, True, 5)
+    down = 40 if exponent > 0 else 0
+    want = np.ldexp(x.double().numpy() @ plain_int4(x, code, scales, zero, group)[1].T, exponent - down)
+    assert np.abs(want).max() < 2.0 ** 127
+    got = ops.gemm_int4_bf16(guarded(torch.ldexp(x.float(), torch.tensor(exponent)).to(torch.bfloat16)), guarded(packed),
+                             guarded(torch.ldexp(scales, torch.tensor(-down))), group, guarded(zero), torch.float32)
+    assert np.array_equal(f64(got), want)
+
+
+@pytest.mark.parametrize("rows, n, k, group", FORMS)
+@pytest.mark.parametrize("scale", [2.0 ** -12, 2.0 ** -30])
+def test_products_in_4_bits_of_the_largest_numbers(ops, rows, n, k, group, scale):
+    """Every x is the largest bfloat16 number, of one sign in the first row; up to K / 2^12 of float32's range goes into a sum of |scale x|.  Bounds
+    as for ordinary x: an addition is off by half a step of a partial sum."""
+    _, code, packed, _, zero = int4_inputs(rows, n, k, group, True, torch.float32, False, 6)
+    g = torch.Generator().manual_seed(7)
+    x = torch.full((rows, k), torch.finfo(torch.bfloat16).max, dtype=torch.bfloat16)
+    x[1:] *= (torch.randint(0, 2, (rows - 1, k), generator=g) * 2 - 1).to(torch.bfloat16)
+    scales = scale * (0.5 + 0.5 * torch.rand(n, -(-k // group), generator=g))
+    xd, w, s, z = plain_int4(x, code, scales, zero, group)
+    want, size = xd @ w.T, np.abs(xd) @ (s * (32.0 + code.double().numpy() + z)).T
+    bound = F32_STEP * (128 + 4 + -(-k // 128) + 8) * size
+    got = f64(ops.gemm_int4_bf16(guarded(x), guarded(packed), guarded(scales), group, guarded(zero), torch.float32))
+    fits = np.abs(want) + bound < np.finfo(np.float32).max
+    assert fits[1:].all() and fits.any(0).all() if scale < 2.0 ** -20 else fits.any()
+    assert (np.abs(got - want)[fits] <= bound[fits]).all()
+    assert np.isinf(got[np.abs(want) - bound > np.finfo(np.float32).max]).all()
+
+
+@pytest.mark.parametrize("rows, n, k, group", FORMS)
+def test_products_in_4_bits_at_the_small_end(ops, rows, n, k, group):
+    """x of some 2^-118: results are off by what ordinary ones are and, an operation, 2^12 times half the least step of float32 (2^-149), times the
+    scale below 1 where it is not the last one."""
+    x, code, packed, scales, zero = int4_inputs(rows, n, k, group, True, torch.float32, False, 8)
+    x = torch.ldexp(x.float(), torch.tensor(-118)).to(torch.bfloat16)
+    xd, w, s, z = plain_int4(x, code, scales, zero, group)
+    count = 128 + 4 + -(-k // 128) + 8
+    bound = F32_STEP * count * (np.abs(xd) @ (s * (32.0 + code.double().numpy() + z)).T) + 2.0 ** -138 * (k + count)
+    got = f64(ops.gemm_int4_bf16(guarded(x), guarded(packed), guarded(scales), group, guarded(zero), torch.float32))
+    assert (np.abs(got - xd @ w.T) <= bound).all()
 
 
 # ---------------------------------------------------------------- attention over pages that the batch shares
