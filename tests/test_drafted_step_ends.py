@@ -25,6 +25,11 @@ def test_the_ends_of_a_drafted_steps_operators_pass_on_the_cpu_build(units):
     env.pop("RI_EMU_COMPUTE_UNITS", None)
     if units:
         env["RI_EMU_COMPUTE_UNITS"] = units
-    run = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider", os.path.join(HERE, "test_drafted_step_ends_gpu.py")],
-                         capture_output=True, text=True, env=env, cwd=ROOT, timeout=600)
+    args = [sys.executable, "-m", "pytest", "-q", "-x", "-p", "no:cacheprovider", os.path.join(HERE, "test_drafted_step_ends_gpu.py")]
+    try:
+        import xdist  # noqa: F401
+        args += ["-n", str(max(1, min(4, (os.cpu_count() or 2) // 2)))]
+    except ImportError:
+        pass
+    run = subprocess.run(args, capture_output=True, text=True, env=env, cwd=ROOT, timeout=600)
     assert run.returncode == 0 and " passed" in run.stdout and "[emu]" not in run.stderr, run.stdout[-3000:] + run.stderr[-3000:]

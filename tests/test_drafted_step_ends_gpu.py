@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, F32_STEP, PAGE, SharedCase, _guarded_buffers_go_back, drafted, f64, guarded, i32,  # noqa: F401
-                                           int4_inputs, ops, plain_int4, pytestmark, verify)
+                                           int4_inputs, ops, plain_int4, pytestmark, softmax, verify)
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -322,3 +322,27 @@ def test_draft_logits_of_tokens_that_are_no_drafts_are_not_read(ops, vocab):
               args[1].data_ptr(), ws.data_ptr(), 1, 3, vocab, 1.0, 0)
     want = verify(ops, logits, draft, tokens, [3], u, 1.0)
     assert np.array_equal(accepted.numpy(), want[0]) and np.array_equal(out.numpy(), want[1])
+
+
+@pytest.mark.parametrize("p_row, q_row, temperature", [([1.0, 0.2, -1.5], [-1.2, 0.8, 0.5], 1.0)] if EMULATED else
+                         [([1.0, 0.2, -1.5], [-1.2, 0.8, 0.5], 1.0), ([0.5, -2.0, 1.0, 0.3, 2.5], [2.0, 1.0, 0.5, -1.0, 0.0], 0.7),
+                          ([3.0, 0.0, 0.0, 0.0, -1.0, 1.0], [0.0, 0.0, 1.0, 2.0, 0.0, 0.0], 1.5)])
+def test_the_first_token_put_out_has_the_targets_probabilities(ops, p_row, q_row, temperature):
+    """Every pair of numbers of a grid and every draft, weighed by the draft's distribution.  Of g midpoints as many lie below a border as its
+    place times g, give or take one half.  So a draft's share of acceptances is off by 1 / 2g at most, a token's share of the draws from what
+    is left, between two borders, by 1 / g, and the token t's probability by (q_t + r_t) / 2g + (1 - acceptance) / g, with r what is left, made a
+    distribution.  Neither drawing from p after a fall nor letting every draft stand would keep within that."""
+    vocab, grid = len(p_row), 16 if EMULATED else 64
+    p_row, q_row = np.array(p_row, dtype=np.float32), np.array(q_row, dtype=np.float32)
+    p, q = softmax(p_row, temperature), softmax(q_row, temperature)
+    left = np.maximum(p - q, 0.0)
+    fallen, left = left.sum(), left / left.sum()
+    bound = (q + left) / (2 * grid) + fallen / grid + 1e-9
+    for wrong in (np.minimum(p, q) + fallen * p, q, p[::-1]):
+        assert (np.abs(wrong - p) > 2 * bound).any()
+    cells = [(d, a, b) for d in range(vocab) for a in range(grid) for b in range(grid)]
+    tokens = np.array([[0, d] for d, _, _ in cells]).reshape(-1)
+    u = np.array([[(a + 0.5) / grid, (b + 0.5) / grid] for _, a, b in cells]).reshape(-1)
+    _, out = verify(ops, np.tile(p_row, (2 * len(cells), 1)), np.tile(q_row, (2 * len(cells), 1)), tokens, [2] * len(cells), u, temperature)
+    found = np.bincount(out[::2], weights=np.repeat(q, grid * grid) / grid ** 2, minlength=vocab)
+    assert (np.abs(found - p) <= bound).all(), (found, p, bound)
