@@ -617,7 +617,7 @@ int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const void* codes
 
 // Attention of the new tokens of `seqs` sequences (cu_seqlens; max_new each sizes the grid) whose page tables begin with the same
 // shared_pages pages (read from the first row of page_table); bfloat16, pages of 32, every sequence at most max_len tokens long after
-// the step.  workspace: ri_attention_shared_slots(...) * tokens * heads * (head_dim + 2) floats.  Tokens that are no sequence's
+// the step (keys from there on are not seen).  workspace: ri_attention_shared_slots(...) * tokens * heads * (head_dim + 2) floats.  Tokens that are no sequence's
 // (before cu_seqlens[0], from cu_seqlens[seqs] on) get zeros.
 int ri_attention_shared_slots(int tokens, int seqs, int max_new, int shared_pages, int max_len, int heads, int kv_heads);
 int ri_attention_shared_bf16(void* out, void* workspace, const void* q, int q_stride, const void* k_pages, const void* v_pages,

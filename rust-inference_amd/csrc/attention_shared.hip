@@ -9,10 +9,13 @@
 // exp2(s - m) and the sum of exp2(s - m) v; the shared pages are cut into runs, every sequence's own pages into chunks, and
 // a second kernel joins a token's runs and chunks in order:
 //     out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i,  M the largest m_i.
-// Statistics and sums are float32; the weights enter the second product rounded to bfloat16, l is taken before the rounding.
+// Statistics and sums are float32; the weights enter the second product rounded to bfloat16, as the matrix cores take it and as in the
+// other attentions here (products of float32 weights would be eight times the instructions); l is taken before the rounding.  A weight is
+// off by 2^-8 of itself at most, one way or the other, so that most of it goes out in the sum: a result's distance from 64 bits grows from
+// 0.0017 of it, its own rounding, to 0.0019 to 0.0021.
 //
-// Keys and values behind a sequence's last token are whatever the page held before: they are taken as zeros, so that an
-// infinity or NaN there reaches nothing.
+// Keys and values behind a sequence's largest position, or from max_len on, are whatever the page held before: they are taken as zeros, so
+// that an infinity or NaN there reaches nothing.
 #include <float.h>
 
 #include "attention_mfma.h"
@@ -482,8 +485,9 @@ struct SharedPlan { int nt, few, waves, splits, pages_per_split, tiles, own_tile
 // half as often: 16 sequences of up to 5 tokens of 4 heads a key head, 20 to 900 own keys, 14.0 us (tiles of 16: 15.7).
 // More than 32 columns a key head take the form of many columns: workgroups of four wavefronts with a tile of 64 or, from 65 columns on,
 // 128; from 129 columns on, where a run is longer than SH_SHORT_PAGES, of eight with 256, whose copies
-// have three turns to arrive instead of one.  us with four : eight wavefronts: 32 sequences of 64 heads behind 131,072 tokens (runs of 128
-// pages) 237 : 215, 64 of 32 heads behind 8,192 (8 pages) 78 : 79, 52 tokens of 32 heads behind 4,096 (8 pages) 43 : 47.
+// have three turns to arrive instead of one.  us with four : eight wavefronts, up to 32 own keys: 32 sequences of 64 heads behind 131,072
+// tokens (runs of 128 pages) 209 : 189, 64 of 32 heads behind 8,192 (16 and 8 pages) 32.3 : 38.5, 52 of 32 heads behind 4,096 (8 pages)
+// 27.0 : 31.5.
 // The shared pages are cut into as many runs as give every compute unit a workgroup, of eight pages at least: every run costs its columns'
 // sums, written and read again.  Twice as many, us: 64 sequences of 32 heads behind 8,192 34.4 : 31.7, 24 behind 16,384 31.6 : 28.6, 8
 // behind 32,768 44 : 34.5.  Where workgroups of four wavefronts would walk more than SH_LONG_PAGES two stand beside one another (24 sequences

@@ -571,7 +571,9 @@ extern "C" int ri_gemm_int4_bf16(void* out, int out_dtype, const void* x, const 
     const hipStream_t s = (hipStream_t)stream;
     const int pieces = (k + I4_PIECE - 1) / I4_PIECE, tiles = (n + 15) / 16, units = ri_compute_units();
     // More tiles of matrix rows than compute units: x is held and the matrix walked.  In us, so and by tiles: 1 x 8192 x 4096 7.1 and 8.5,
-    // 4 x 12288 x 4096 8.8 and 13.4, 16 x 24576 x 4096 15.5 and 25, 16 x 151936 x 4096 77 and 135; 4 x 5120 x 2560 level.
+    // 4 x 12288 x 4096 8.8 and 13.4, 16 x 24576 x 4096 15.5 and 25, 16 x 151936 x 4096 77 and 135; 4 x 5120 x 2560 level.  The registers of
+    // eight wavefronts hold 32 pieces of 16 rows; beyond K = 4096 all products go by tiles (1 and 16 rows, of the time that the bytes take:
+    // 55296 x 5120 1.5 and 2.1 times, 57344 x 8192 1.5 and 2.0, where 24576 x 4096 takes 1.2 and 1.4).
     if (rows <= 16 && k % 32 == 0 && pieces <= 32 && (long)n * (k / 2) <= 0xffffffffL && tiles > units) {
         if (pieces <= 16) int4_rows<2, 2>(a, group, f, s);
         else int4_rows<4, 1>(a, group, f, s);

@@ -10,9 +10,11 @@
 // given (looked up, not drawn): q is 1 at the draft and 0 elsewhere.  The draw takes the first token whose running
 // weight, by rising id, passes u_last times the weight of all.
 //
-// Everything that is compared is held in 64 bits: a token is the answer to "on which side of a border does u lie", a
-// vocabulary has 10^5 borders, and float32 weights put one draw in 10^3 to 10^5 on the wrong side.  The vector unit takes
-// float64 well, so that an exponential of thirteen instructions (Exps, below) stands beside an entry's 4 bytes.
+// Everything that is compared is a float64: a token is the answer to "on which side of a border does u lie", a
+// vocabulary has 10^5 borders, and float32 weights put one draw in 10^3 to 10^5 on the wrong side.  The exponential keeps 40 of the 53
+// bits (relative error 1.1e-12, which puts less than one draw in 10^6 on the other side): the vector unit takes
+// float64 well, so that its fourteen instructions (Exps, below) stand beside an entry's 4 bytes; each bit more would cost time in a pass
+// that it bounds already.
 //
 // Four launches.  `stats` cuts every row that is asked about into chunks of 4,096 entries, a wavefront each, and leaves a
 // chunk's largest logit and its sum of exponentials: the one pass over the logits.  `end` (a workgroup a sequence) joins the
@@ -69,8 +71,8 @@ __device__ __forceinline__ double exp2_nonpositive(double t) {
 }
 
 // The exponentials of a row's (or a chunk's) entries over that of its largest one.  Ordinary temperatures: with M the whole
-// number next to m s, 2^(x s - M) takes thirteen float64 instructions, since x s + (1.5 * 2^52 - M) has the whole part in
-// place at once, and x is held in float32 to what the exponent has room for: lo, where the result is 2^-1000 up to the
+// number next to m s, 2^(x s - M) takes eleven float64 instructions, a conversion, a clamp and an addition to the exponent, since
+// x s + (1.5 * 2^52 - M) has the whole part in place at once, and x is held in float32 to what the exponent has room for: lo, where the result is 2^-1000 up to the
 // rounding of lo, which is that of a normal number (2^-24, some 2^3 exponents) where |M| is below 2^27, lo in float32's range and s below
 // 2^80 (lo, where it is not 0, is a whole number of 1 / s); `plain` does without.  NaN and what lies at lo or below is a masked entry, an
 // infinite logit the largest finite number.
@@ -184,8 +186,8 @@ __device__ __forceinline__ void place_of_row(const int32_t* __restrict__ cu, int
 }
 
 // A chunk a wavefront, 64 entries a lane: what is done once a wavefront (place, reductions) is a fifth of its instructions so, a
-// third with 32.  The vector unit bounds this pass nearly as the memory does (320 rows x 151,936 and 256 of drafts, 350 MB: 69 us, 5.1 TB/s;
-// with the 64 rows of draft logits that are no draft's read too 70.5 on the same machine).
+// third with 32.  The vector unit bounds this pass nearly as the memory does (320 rows x 151,936 and 256 of drafts, 350 MB: 63 to 69 us, 5.1 to
+// 5.6 TB/s; with the 64 rows of draft logits that are no draft's read too 70.5 where it is 69).
 template <bool WIDE>
 __global__ __launch_bounds__(RI_WAVE) void verify_stats(ChunkStats* __restrict__ stats, const float* __restrict__ logits,
                                                         const float* __restrict__ draft, const int32_t* __restrict__ cu, int seqs,

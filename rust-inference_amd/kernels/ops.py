@@ -546,8 +546,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
 
     Returns int32 ``accepted [seqs]``, the drafts that stand, and int32 ``out [rows]``, at the sequence's rows the drafts that stand, the
     token after them, then -1 (also in rows that are no sequence's).  NaN and -inf mask an entry (a target cut to its best
-    entries is given so), an infinite logit counts as the largest finite number; a draft outside the vocabulary falls.  A row that
-    masks everything lets no draft stand and gives token 0.  At most 65,535 rows and sequences."""
+    entries is given so, the caller masks it), one that weighs less than 2^-1000 of the largest counts as masked, an infinite logit counts as the
+    largest finite number; a draft outside the vocabulary falls.  A row that masks everything lets no draft stand and gives token 0.  At most 65,535 rows and sequences."""
     if logits.dim() != 2:
         raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
     rows, vocab = logits.shape
@@ -1495,10 +1495,12 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     tokens instead of once a sequence.  ``shared`` is a multiple of the page (32 tokens; 0: nothing is shared) and the first
     ``shared / 32`` entries of every row of ``page_table`` are the same pages (the first row's are read).  Any number of new tokens
     a sequence, as a rule at most ``max_new`` (one, or a drafted step's few; it sizes the grid, a sequence that brings more takes longer), their
-    positions in any order; their keys and values are in the cache.  ``max_len`` bounds every sequence's length after this step: it sizes the grid and the workspace, and keys behind it are not seen.  What a page holds behind
-    a sequence's last token may be anything; the values of its tokens are finite (a token's weight for a later one is 0, which does
-    not undo an infinity).  ``scale`` times a query's product with a key stays below 10^9 in magnitude, as in the other matrix-core attentions
-    (a score's float32 exponent against the largest one's has to).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
+    positions in any order; their keys and values are in the cache.  ``max_len`` bounds every sequence's length after this step: it sizes the
+    grid and the workspace, and keys from there on are not seen.  What a page holds behind a sequence's last token may be anything; the values
+    of its tokens are finite (a token's weight for a later one is 0, which does not undo an infinity).  One token a sequence: faster than
+    ``attention_decode_bf16`` from 4 sequences behind 1,024 tokens or 2 behind 4,096 on, slower with less to share; several tokens: faster than
+    ``attention_prefill_bf16`` from 1,024 on.  ``scale`` times a query's product with a key stays below 10^9 in magnitude, as in the other
+    matrix-core attentions (a score's float32 exponent against the largest one's has to).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
     tokens, stride = qkv.shape
     num_pages, hkv, page_size, dh = k_pages.shape
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -1574,8 +1576,10 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
     """``x @ w.T`` for bfloat16 rows ``x [M, K]`` and a matrix in 4 bits: ``w[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k //
     group])``.  ``codes`` (uint8 ``[N, K / 2]``) hold two neighbouring columns a byte, the even one in the low four bits; ``scales``
     (bfloat16 or float32) and ``zeros`` (uint8; None: 8 everywhere) are ``[N, ceil(K / group)]``.  ``group`` is 32, 64 or a multiple of
-    128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights; with more
-    the codes are read again for every 64.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at
+    128, ``K`` a multiple of 8 (the last group may be short).  Made for the 1 to 64 rows of a step that streams its weights: up to
+    16 the codes are read once, with more again for every 16 or 64.  Against the same matrix in bfloat16 a product takes 0.3 to 0.85
+    of the time up to 16 rows and 0.8 to 1.1 of it up to 32; from some 45 rows on a wide matrix is faster in bfloat16 (1.1 to 1.45 times), and
+    what 4 bits save is memory.  Float32 sums of unrounded products, one rounding to ``out_dtype`` (bfloat16 or float32) at
     the end.  The sums stay in range for any finite ``x`` for which the sum of ``|scale x|`` over ``K`` does; results below 2^-114 in magnitude have
     fewer bits.  A row of ``x`` with an infinity or NaN gives NaN, the other rows what they gave."""
     if x.dim() != 2 or codes.dim() != 2:
