@@ -291,10 +291,9 @@ def _on_current_device(first: torch.Tensor, *others) -> None:
         raise KernelError(f"the operands lie on {first.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
 
 
-def _in_32_bits(what: str, *sizes: int) -> None:
-    """The sizes fit the C interface's numbers (ctypes would cut off what lies above 32 bits without a word)."""
-    if max(sizes) > 0x7FFFFFFF:
-        raise ShapeError(f"{what} of {' x '.join(str(s) for s in sizes)}: at most 2^31 - 1 each")
+def _beyond_32_bits(what: str, *sizes: int) -> ShapeError:
+    """For sizes that the C interface's numbers do not hold (ctypes would cut off what lies above 32 bits without a word)."""
+    return ShapeError(f"{what} of {' x '.join(str(s) for s in sizes)}: at most 2^31 - 1 each")
 
 
 # ---------------------------------------------------------------- row-wise
@@ -537,7 +536,7 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     ``cu_seqlens[b]..cu_seqlens[b + 1]``: its last known token, then its drafts, none of them or any number) and whose logits
     are all wanted.  Row ``r`` of float32 ``logits [rows, vocab]`` is what follows token ``r`` and judges the draft
     ``tokens[r + 1]``: with ``p = softmax(logits[r] / temperature)`` and ``q`` the distribution the draft was drawn from it
-    stands if ``uniform[r] * q(draft) < p(draft)``.  ``draft_logits`` (float32 ``[rows, vocab]``): row ``j`` is what ``tokens[j]`` was
+    stands if ``uniform[r] * q(draft) < p(draft)`` (``uniform``: float32 ``[rows]``, from 0 to below 1).  ``draft_logits`` (float32 ``[rows, vocab]``): row ``j`` is what ``tokens[j]`` was
     drawn from, at the same temperature (rows of tokens that are no drafts are not read); None: the drafts were not drawn
     (looked up), ``q`` is 1 at the draft.  Behind the drafts that stand comes one more token, drawn with the number of the
     sequence's last row: from ``max(p - q, 0)`` where a draft fell, else from the last row's ``p``; the first token whose running
@@ -547,7 +546,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     Returns int32 ``accepted [seqs]``, the drafts that stand, and int32 ``out [rows]``, at the sequence's rows the drafts that stand, the
     token after them, then -1 (also in rows that are no sequence's).  NaN and -inf mask an entry (a target cut to its best
     entries is given so, the caller masks it), one that weighs less than 2^-1000 of the largest counts as masked, an infinite logit counts as the
-    largest finite number; a draft outside the vocabulary falls.  A row that masks everything lets no draft stand and gives token 0.  At most 65,535 rows and sequences."""
+    largest finite number; a draft outside the vocabulary falls.  A row that masks everything lets no draft stand and gives token 0.  At most 65,535
+    rows and sequences."""
     if logits.dim() != 2:
         raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
     rows, vocab = logits.shape
@@ -556,7 +556,8 @@ def verify_drafts(logits: torch.Tensor, tokens: torch.Tensor, cu_seqlens: torch.
     seqs, temperature = cu_seqlens.shape[0] - 1, float(temperature)
     if rows < 1 or vocab < 1:
         raise ShapeError(f"logits must be [rows, vocab], got {list(logits.shape)}")
-    _in_32_bits("logits of rows and a vocabulary", rows, vocab)
+    if (rows | vocab) >> 31:
+        raise _beyond_32_bits("logits of rows and a vocabulary", rows, vocab)
     if temperature > 0 and uniform is None:
         raise ShapeError("a temperature above 0 wants uniform numbers, one a row")
     _on_current_device(logits, tokens, cu_seqlens, uniform, draft_logits)
@@ -1500,7 +1501,8 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     of its tokens are finite (a token's weight for a later one is 0, which does not undo an infinity).  One token a sequence: faster than
     ``attention_decode_bf16`` from 4 sequences behind 1,024 tokens or 2 behind 4,096 on, slower with less to share; several tokens: faster than
     ``attention_prefill_bf16`` from 1,024 on.  ``scale`` times a query's product with a key stays below 10^9 in magnitude, as in the other
-    matrix-core attentions (a score's float32 exponent against the largest one's has to).  ``q_off`` as in ``attention``.  Tokens outside ``cu_seqlens`` get zeros."""
+    matrix-core attentions (a score's float32 exponent against the largest one's has to).  ``q_off`` as in ``attention``.  Tokens outside
+    ``cu_seqlens`` get zeros."""
     tokens, stride = qkv.shape
     num_pages, hkv, page_size, dh = k_pages.shape
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
@@ -1516,7 +1518,8 @@ def attention_shared_bf16(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table
     reach = page_table.shape[1] * page_size
     if shared > reach or not 1 <= max_len <= reach:           # (before the workspace is sized by them)
         raise ShapeError(f"attention: {shared} shared tokens, sequences of up to {max_len}, tables of {reach}")
-    _in_32_bits("tables of tokens, queries of tokens and columns, pages", reach, tokens, stride, num_pages)
+    if (reach | tokens | stride | num_pages) >> 31:
+        raise _beyond_32_bits("tables of tokens, queries of tokens and columns, pages", reach, tokens, stride, num_pages)
     max_new = min(int(max_new), tokens)
     _on_current_device(qkv, k_pages, v_pages, cu_seqlens, tok_pos, page_table)
     args = (_dev(qkv, "qkv", torch.bfloat16) + 2 * int(q_off), stride, _dev(k_pages, "k_pages", torch.bfloat16),
@@ -1589,9 +1592,11 @@ def gemm_int4_bf16(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, g
         raise ShapeError(f"groups of {group} columns: 32, 64 and multiples of 128 are taken")
     if m < 1 or n < 1 or k < 8 or k % 8:
         raise ShapeError(f"a product of {m} rows, {n} columns and k {k}: at least one each, k a multiple of 8")
-    _in_32_bits("a product of rows, columns and k", m, n, k)
+    if (m | n | k) >> 31:
+        raise _beyond_32_bits("a product of rows, columns and k", m, n, k)
     groups = -(-k // group)
-    group = min(group, -(-k // 128) * 128)                    # (a longer one is the same one group, and the kernel's number has 32 bits)
+    if group > 128 and group > k:                             # (a longer one is the same one group, and the kernel's number has 32 bits)
+        group = -(-k // 128) * 128
     _on_current_device(x, codes, scales, zeros)
     out = torch.empty((m, n), dtype=out_dtype, device=x.device)
     _call("ri_gemm_int4_bf16", _dev(out, "out"), code(out_dtype), _dev(x, "x", torch.bfloat16), _dev(codes, "codes", torch.uint8, (n, k // 2)),

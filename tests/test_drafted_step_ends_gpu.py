@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_drafted_step_kernels_gpu import (BF16_STEP, EMULATED, F32_STEP, PAGE, SharedCase, _guarded_buffers_go_back, drafted, f64, guarded, i32,  # noqa: F401
-                                           int4_inputs, ops, plain_int4, pytestmark, softmax, verify)
+                                           int4_inputs, ops, plain_int4, pytestmark, softmax, starts, verify)
 
 
 # ---------------------------------------------------------------- products with a matrix in 4 bits
@@ -203,6 +203,19 @@ def test_attention_over_shared_pages_of_scores_up_to_a_billion(ops, heads):
     c.check(c.run(ops))
 
 
+@pytest.mark.parametrize("heads", [4, 40])
+def test_attention_over_shared_pages_leaves_rows_before_the_sequences_at_zero(ops, heads):
+    """Two rows of NaN before the first sequence and one behind the last, which are no sequence's; the others as without them."""
+    c = SharedCase([(2, 10), (1, 35), (3, 300)], 96, heads, 2, 64, seed=18)
+    want = c.run(ops)
+    c.check(want)
+    pad = torch.full((2, c.qkv.shape[1]), float("nan"), dtype=torch.bfloat16)
+    c.qkv, c.pos = torch.cat([pad, c.qkv, pad[:1]]), [3, 10 ** 9] + c.pos + [-2]
+    got = ops.attention_shared_bf16(guarded(c.qkv), guarded(c.k), guarded(c.v), i32(2 + starts(c.counts)), i32(c.pos), guarded(c.table), 3, c.max_new,
+                                    c.shared, c.max_len, heads, 2, 64, c.scale)
+    assert (f64(got)[[0, 1, 8]] == 0).all() and torch.equal(got[2:8], want)
+
+
 @pytest.mark.parametrize("which", ["k", "v", "qkv"])
 def test_attention_over_shared_pages_refuses_what_does_not_start_on_16_bytes(ops, which):
     from rust_inference_amd.errors import KernelError
@@ -346,3 +359,71 @@ def test_the_first_token_put_out_has_the_targets_probabilities(ops, p_row, q_row
     _, out = verify(ops, np.tile(p_row, (2 * len(cells), 1)), np.tile(q_row, (2 * len(cells), 1)), tokens, [2] * len(cells), u, temperature)
     found = np.bincount(out[::2], weights=np.repeat(q, grid * grid) / grid ** 2, minlength=vocab)
     assert (np.abs(found - p) <= bound).all(), (found, p, bound)
+
+
+# ---------------------------------------------------------------- streams and graphs
+def step_inputs(seed, new, own):
+    """The device operands of a step: attention of ``new`` tokens a sequence behind 128 shared ones, a product, a verification."""
+    c = SharedCase([(n, m) for n, m in zip(new, own)], 128, 8, 2, 64, seed=seed, table_spare=24 - -(-max(own) // PAGE))
+    x, _, packed, scales, zero = int4_inputs(6, 40, 512, 64, True, torch.bfloat16, False, seed)
+    logits, draft, tokens, u = drafted(new, 5000, 1.0, True, seed)
+    f = lambda a: torch.tensor(a, dtype=torch.float32, device="cuda:0")  # noqa: E731
+    return [t.to("cuda:0") for t in (c.qkv, c.table, x, packed, scales, zero)] + [f(logits), f(draft), f(u), i32(tokens), i32(c.pos),
+                                                                                  i32(starts(new))], (c.k.to("cuda:0"), c.v.to("cuda:0"))
+
+
+def step_calls(ops, a, pages, max_new, max_len):
+    qkv, table, x, packed, scales, zero, logits, draft, u, tokens, pos, cu = a
+    return [ops.attention_shared_bf16(qkv, *pages, cu, pos, table, 3, max_new, 128, max_len, 8, 2, 64, 0.125),
+            ops.gemm_int4_bf16(x, packed, scales, 64, zero), *ops.verify_drafts(logits, tokens, cu, u, 0.8, draft),
+            *ops.verify_drafts(logits, tokens, cu, None, 0.0)]
+
+
+@pytest.mark.skipif(EMULATED, reason="streams")
+def test_two_steps_at_once_on_two_streams(ops):
+    """Neither waits for the other; each gives what it gives alone."""
+    cases = [step_inputs(41, [2, 1, 3], [40, 600, 3]), step_inputs(42, [1, 4, 1], [500, 90, 33])]
+    want = [[t.clone() for t in step_calls(ops, a, p, 4, 128 + 700)] for a, p in cases]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for i, (a, p) in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step_calls(ops, a, p, 4, 128 + 700))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, w) for step in got[i] for g, w in zip(step, want[i]))
+
+
+@pytest.mark.skipif(EMULATED, reason="graphs")
+def test_a_captured_step_answers_other_lengths_positions_and_counts(ops):
+    """One graph, captured for two tokens a sequence, replayed over steps whose sequences bring others in number, more than two among them, at
+    other positions: every replay gives the eager bits of a call with the same bounds."""
+    pages = None
+    steps = []
+    for seed, new, own in ((51, [2, 2, 2], [40, 600, 3]), (52, [1, 4, 1], [500, 90, 33]), (53, [6, 0, 0], [700, 1, 1]), (54, [0, 1, 5], [2, 1, 321])):
+        a, pages = step_inputs(seed, new, own)
+        steps.append((a, pages))
+    most = max(p[0].shape[0] for _, p in steps)
+    held_pages = [torch.zeros((most, *t.shape[1:]), dtype=t.dtype, device=t.device) for t in pages]
+    held = [t.clone() for t in steps[0][0]]
+    def put(a, p):
+        for h, t in zip(held, a):
+            h.copy_(t)
+        for h, t in zip(held_pages, p):
+            h[:t.shape[0]].copy_(t)
+    eager = []
+    for a, p in steps:
+        put(a, p)
+        eager.append([t.clone() for t in step_calls(ops, held, held_pages, 2, 128 + 700)])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step_calls(ops, held, held_pages, 2, 128 + 700)
+    for turn in range(9):
+        i = turn * 3 % 4
+        put(*steps[i])
+        graph.replay()
+        torch.ones(1000, device="cuda:0").sum()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(out, eager[i])), (turn, i)
