@@ -97,6 +97,22 @@ def test_products_in_4_bits_at_the_small_end(ops, rows, n, k, group):
     assert (np.abs(got - xd @ w.T) <= bound).all()
 
 
+def off_its_start(t, by):
+    """The same numbers behind ``by`` others of a larger tensor."""
+    whole = torch.zeros(t.numel() + by, dtype=t.dtype)
+    whole[by:] = t.reshape(-1)
+    return guarded(whole)[by:].view(t.shape)
+
+
+@pytest.mark.parametrize("rows, n, k, group", FORMS)
+def test_products_in_4_bits_of_operands_that_start_anywhere(ops, rows, n, k, group):
+    """Codes on a 4-byte boundary and no larger one, scales and zero points on one of their own size: the same bits."""
+    x, _, packed, scales, zero = int4_inputs(rows, n, k, group, True, torch.bfloat16, False, 9)
+    want = ops.gemm_int4_bf16(guarded(x), guarded(packed), guarded(scales), group, guarded(zero), torch.float32)
+    got = ops.gemm_int4_bf16(guarded(x), off_its_start(packed, 4), off_its_start(scales, 1), group, off_its_start(zero, 3), torch.float32)
+    assert torch.equal(got, want)
+
+
 # ---------------------------------------------------------------- attention over pages that the batch shares
 @pytest.mark.parametrize("change", [dict(max_len=2 ** 32 + 100), dict(max_len=2 ** 40), dict(shared=2 ** 37 + 64), dict(shared=2 ** 40)])
 def test_attention_over_shared_pages_refuses_lengths_that_no_table_holds(ops, change):
@@ -359,6 +375,19 @@ def test_the_first_token_put_out_has_the_targets_probabilities(ops, p_row, q_row
     _, out = verify(ops, np.tile(p_row, (2 * len(cells), 1)), np.tile(q_row, (2 * len(cells), 1)), tokens, [2] * len(cells), u, temperature)
     found = np.bincount(out[::2], weights=np.repeat(q, grid * grid) / grid ** 2, minlength=vocab)
     assert (np.abs(found - p) <= bound).all(), (found, p, bound)
+
+
+@pytest.mark.parametrize("vocab", [4100, 9000])
+@pytest.mark.parametrize("temperature", [0.8, 0.0])
+def test_drafts_are_verified_from_logits_that_start_anywhere(ops, vocab, temperature):
+    """On a 4-byte boundary and no larger one."""
+    counts = [3, 1, 4]
+    logits, draft, tokens, u = drafted(counts, vocab, 0.8, True, 19)
+    want = verify(ops, logits, draft, tokens, counts, u, temperature)
+    for by in ((1, 0), (0, 1), (3, 2)):
+        t = [off_its_start(torch.tensor(a), o) for a, o in zip((logits, draft), by)]
+        got = ops.verify_drafts(t[0], i32(tokens), i32(starts(counts)), off_its_start(torch.tensor(u), 1), temperature, t[1])
+        assert np.array_equal(got[0].cpu().numpy(), want[0]) and np.array_equal(got[1].cpu().numpy(), want[1])
 
 
 # ---------------------------------------------------------------- streams and graphs
